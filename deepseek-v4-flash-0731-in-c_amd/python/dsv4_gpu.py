@@ -32,8 +32,20 @@ class DSV4GLayer(C.Structure):
     ]
 
 
+class DSV4GCache(C.Structure):
+    """Mirror of DSV4GCache (include/dsv4_gpu.h)."""
+
+    _fields_ = [
+        ("pages", _vp), ("ref", _vp), ("table", _vp), ("len", _vp), ("status", _vp),
+        ("n_layers", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+        ("kv_heads", C.c_int), ("k_dim", C.c_int), ("v_dim", C.c_int), ("dtype", C.c_int),
+        ("n_seqs", C.c_int), ("max_pages", C.c_int),
+    ]
+
+
 # (name, argtypes) for the device-pointer ABI; all return int.
 _I, _F, _Z = C.c_int, C.c_float, C.c_size_t
+_CP = C.POINTER(DSV4GCache)
 _SIGS = {
     "dsv4g_quant_fp8_act": [_vp, _vp, _vp, _I, _I, _vp],
     "dsv4g_dequant_fp4": [_vp, _vp, _vp, _I, _I, _vp],
@@ -75,11 +87,64 @@ _SIGS = {
     "dsv4g_hc_post": [_vp, _vp, _vp, _vp, _I, _I, _I, _vp],
     "dsv4g_ffn_step": [_vp, _vp, _vp, _vp, _vp, C.POINTER(DSV4GLayer), _vp, _I, _I, _I, _F, _F,
                        _vp, _Z, _vp, _vp, _vp],
+    "dsv4g_logprobs": [_vp, _vp, _vp, _vp, _vp, _vp, _I, _I, _I, _Z, _vp, _I, _F, _vp, _Z, _vp],
+    "dsv4g_cache_init": [_CP, _vp],
+    "dsv4g_cache_status": [_vp, _CP, _vp],
+    "dsv4g_cache_reserve": [_CP, _vp, _vp, _I, _vp, _Z, _vp],
+    "dsv4g_cache_append": [_CP, _I, _vp, _Z, _vp, _Z, _I, _vp, _vp, _I, _I, _vp],
+    "dsv4g_cache_fork": [_CP, _vp, _vp, _I, _vp],
+    "dsv4g_cache_free": [_CP, _vp, _vp, _I, _vp],
+    "dsv4g_cache_compact": [_CP, _vp, _vp, _Z, _vp],
+    "dsv4g_attention": [_vp, _Z, _vp, _vp, _Z, _I, _CP, _I, _I, _vp, _vp, _I, _I, _I, _I, _F, _I,
+                        _vp, _vp, _Z, _vp],
 }
 
 
 def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+# ---- argument checks of the entries that take whole tensors
+def _same_device(who, *tensors):
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and (t.device != dev or not t.is_cuda):
+            raise ValueError(f"{who}: tensors must be on one GPU")
+
+
+def _int32(who, t, n):
+    import torch
+    if t is not None and (t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous()):
+        raise ValueError(f"{who}: contiguous int32 tensor of {n} entries needed, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+
+
+def _act_dtype(who, *tensors):
+    """DSV4G_DT_F32 or _BF16 of float32 / bfloat16 tensors of one type."""
+    import torch
+    kinds = {t.dtype for t in tensors if t is not None}
+    if kinds == {torch.float32}:
+        return DTYPE_CODES["F32"]
+    if kinds == {torch.bfloat16}:
+        return DTYPE_CODES["BF16"]
+    raise ValueError(f"{who}: float32 or bfloat16 tensors of one type needed, got {kinds}")
+
+
+def _rows(who, t, heads, dim):
+    """Elements from token to token of [tokens][heads][dim] with whole rows."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1 or \
+            (heads > 1 and t.stride(1) != dim):
+        raise ValueError(f"{who}: [tokens][{heads}][{dim}] with contiguous rows needed, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+def _workspace(workspace, need, device):
+    """The caller's workspace if it is large enough, else a fresh one."""
+    import torch
+    if workspace is None or workspace.nbytes < need:
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+    return workspace
 
 
 class GpuLib:
@@ -97,6 +162,13 @@ class GpuLib:
         lib.dsv4g_moe_batch_workspace_bytes.argtypes = [C.POINTER(DSV4GLayer), _I]
         lib.dsv4g_ffn_step_workspace_bytes.restype = C.c_size_t
         lib.dsv4g_ffn_step_workspace_bytes.argtypes = [C.POINTER(DSV4GLayer), _I, _I]
+        for name, args in (("dsv4g_logprobs_workspace_bytes", [_I, _I, _I]),
+                           ("dsv4g_cache_page_bytes", [_CP]),
+                           ("dsv4g_cache_workspace_bytes", [_CP]),
+                           ("dsv4g_attention_workspace_bytes", [_CP, _I, _I, _I, _I, _I])):
+            fn = getattr(lib, name)
+            fn.argtypes = args
+            fn.restype = C.c_size_t
         for name, args in _SIGS.items():
             fn = getattr(lib, name)
             fn.argtypes = args
@@ -203,6 +275,167 @@ class GpuLib:
         idx = torch.empty(n, dtype=torch.int32, device=logits.device) if idx is None else idx
         self._call("dsv4g_argmax", _ptr(idx), _ptr(logits), vocab, n, vocab, self._stream())
         return idx
+
+    def logprobs_workspace_bytes(self, vocab, n, top=0):
+        return int(self.lib.dsv4g_logprobs_workspace_bytes(vocab, n, top))
+
+    def logprobs(self, logits, tokens=None, top=0, scale=1.0, workspace=None):
+        """dsv4g_logprobs over the rows of logits [n][vocab] (float32 or
+        bfloat16, rows may be strided) for tokens [n] (int32): (logprob,
+        entropy, rank, top_id [n][top], top_logprob [n][top]); without tokens
+        logprob and rank are None, without top the last two are."""
+        import torch
+        if logits.dim() != 2 or logits.stride(1) != 1 or (logits.shape[0] > 1 and
+                                                          logits.stride(0) < logits.shape[1]):
+            raise ValueError("logprobs: logits must be [n][vocab] with contiguous rows")
+        n, vocab = logits.shape
+        dt = _act_dtype("logprobs", logits)
+        _same_device("logprobs", logits, tokens, workspace)
+        _int32("logprobs", tokens, n)
+        with torch.cuda.device(logits.device):
+            need = self.logprobs_workspace_bytes(vocab, n, top)
+            workspace = _workspace(workspace, need, logits.device)
+            f = dict(dtype=torch.float32, device=logits.device)
+            i = dict(dtype=torch.int32, device=logits.device)
+            logprob = rank = ids = top_lp = None
+            entropy = torch.empty(n, **f)
+            if tokens is not None:
+                logprob, rank = torch.empty(n, **f), torch.empty(n, **i)
+            if top:
+                ids, top_lp = torch.empty(n, top, **i), torch.empty(n, top, **f)
+            self._call("dsv4g_logprobs", _ptr(logprob), _ptr(entropy), _ptr(rank), _ptr(ids),
+                       _ptr(top_lp), _ptr(logits), dt, vocab, n, max(logits.stride(0), vocab),
+                       _ptr(tokens), top, scale, _ptr(workspace), workspace.nbytes,
+                       self._stream())
+        return logprob, entropy, rank, ids, top_lp
+
+    # ---- paged cache and the attention over it
+    def cache_workspace_bytes(self, cache):
+        return int(self.lib.dsv4g_cache_workspace_bytes(C.byref(cache.struct)))
+
+    def cache_init(self, cache):
+        """Every sequence empty, every page free."""
+        import torch
+        with torch.cuda.device(cache.device):
+            self._call("dsv4g_cache_init", C.byref(cache.struct), self._stream())
+
+    def cache_status(self, cache):
+        """The cache's sticky status word (0: fine; CACHE_FULL, CACHE_LIST,
+        CACHE_PAGE), cleared."""
+        import torch
+        st = C.c_uint(0)
+        with torch.cuda.device(cache.device):
+            self._call("dsv4g_cache_status", C.byref(st), C.byref(cache.struct), self._stream())
+        return st.value
+
+    def cache_reserve(self, cache, starts, seqs=None, workspace=None):
+        """dsv4g_cache_reserve: room for starts[i + 1] - starts[i] new tokens
+        of each listed sequence (int32 tensors)."""
+        import torch
+        n = starts.numel() - 1
+        _same_device("cache_reserve", cache.pages, starts, seqs, workspace)
+        _int32("cache_reserve", starts, n + 1)
+        _int32("cache_reserve", seqs, n)
+        with torch.cuda.device(cache.device):
+            workspace = _workspace(workspace, self.cache_workspace_bytes(cache), cache.device)
+            self._call("dsv4g_cache_reserve", C.byref(cache.struct), _ptr(seqs), _ptr(starts), n,
+                       _ptr(workspace), workspace.nbytes, self._stream())
+
+    def cache_append(self, cache, layer, k, v, starts, seqs=None):
+        """dsv4g_cache_append: k [tokens][kv_heads][k_dim] and v likewise (None
+        where the values are the keys) into one layer's pages; tokens may be
+        strided."""
+        import torch
+        s = cache.struct
+        n = starts.numel() - 1
+        _same_device("cache_append", cache.pages, k, v, starts, seqs)
+        _int32("cache_append", starts, n + 1)
+        _int32("cache_append", seqs, n)
+        dt = _act_dtype("cache_append", k, v)
+        ks = _rows("cache_append", k, s.kv_heads, s.k_dim)
+        vs = 0 if v is None else _rows("cache_append", v, s.kv_heads, s.v_dim)
+        if v is not None and v.shape[0] != k.shape[0]:
+            raise ValueError("cache_append: k and v of different lengths")
+        with torch.cuda.device(cache.device):
+            self._call("dsv4g_cache_append", C.byref(s), layer, _ptr(k), ks, _ptr(v), vs, dt,
+                       _ptr(seqs), _ptr(starts), n, k.shape[0], self._stream())
+
+    def cache_fork(self, cache, parents, children):
+        """dsv4g_cache_fork: empty sequence children[i] shares parents[i]'s pages."""
+        import torch
+        n = children.numel()
+        _same_device("cache_fork", cache.pages, parents, children)
+        _int32("cache_fork", parents, n)
+        _int32("cache_fork", children, n)
+        with torch.cuda.device(cache.device):
+            self._call("dsv4g_cache_fork", C.byref(cache.struct), _ptr(parents), _ptr(children),
+                       n, self._stream())
+
+    def cache_free(self, cache, seqs, new_len=None):
+        """dsv4g_cache_free: the listed sequences cut back to new_len tokens
+        (None: 0)."""
+        import torch
+        n = seqs.numel()
+        _same_device("cache_free", cache.pages, seqs, new_len)
+        _int32("cache_free", seqs, n)
+        _int32("cache_free", new_len, n)
+        with torch.cuda.device(cache.device):
+            self._call("dsv4g_cache_free", C.byref(cache.struct), _ptr(seqs), _ptr(new_len), n,
+                       self._stream())
+
+    def cache_compact(self, cache, n_used=None, workspace=None):
+        """dsv4g_cache_compact; n_used (int32 [1], optional) takes the number
+        of pages in use."""
+        import torch
+        _same_device("cache_compact", cache.pages, n_used, workspace)
+        _int32("cache_compact", n_used, 1)
+        with torch.cuda.device(cache.device):
+            workspace = _workspace(workspace, self.cache_workspace_bytes(cache), cache.device)
+            self._call("dsv4g_cache_compact", C.byref(cache.struct), _ptr(n_used),
+                       _ptr(workspace), workspace.nbytes, self._stream())
+
+    def attention_workspace_bytes(self, cache, heads, n_seqs, n_tokens, max_q, max_kv):
+        return int(self.lib.dsv4g_attention_workspace_bytes(
+            C.byref(cache.struct), heads, n_seqs, n_tokens, max_q, max_kv))
+
+    def attention(self, cache, layer, q, starts, seqs=None, max_q=None, max_kv=None, scale=None,
+                  window=0, sink=None, out=None, lse=None, with_lse=False, workspace=None):
+        """dsv4g_attention of q [tokens][heads][k_dim] (bfloat16, or float32
+        holding BF16 values; tokens may be strided): out, or (out, lse) with
+        lse given or with_lse. max_q, max_kv: bounds of the listed counts and
+        lengths (default: all tokens, the table's width); scale: k_dim ** -0.5."""
+        import torch
+        s = cache.struct
+        n, tokens = starts.numel() - 1, q.shape[0]
+        heads = q.shape[1] if q.dim() == 3 else 0
+        _same_device("attention", cache.pages, q, starts, seqs, sink, out, lse, workspace)
+        _int32("attention", starts, n + 1)
+        _int32("attention", seqs, n)
+        qs = _rows("attention", q, heads, s.k_dim)
+        dv = s.v_dim or s.k_dim
+        max_q = tokens if max_q is None else max_q
+        max_kv = s.max_pages * s.page_size if max_kv is None else max_kv
+        with torch.cuda.device(cache.device):
+            if out is None:
+                out = torch.empty(tokens, heads, dv, dtype=q.dtype, device=q.device)
+            if lse is None and with_lse:
+                lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
+            dt = _act_dtype("attention", q, out)
+            os_ = _rows("attention", out, heads, dv)
+            for t, size in ((lse, tokens * heads), (sink, heads)):
+                if t is not None and (t.dtype != torch.float32 or t.numel() != size or
+                                      not t.is_contiguous()):
+                    raise ValueError("attention: lse and sink must be contiguous float32, "
+                                     "[tokens][heads] and [heads]")
+            if out.shape[0] != tokens:
+                raise ValueError("attention: out and q of different lengths")
+            workspace = _workspace(workspace, self.attention_workspace_bytes(
+                cache, heads, n, tokens, max_q, max_kv), q.device)
+            self._call("dsv4g_attention", _ptr(out), os_, _ptr(lse), _ptr(q), qs, dt, C.byref(s),
+                       layer, heads, _ptr(seqs), _ptr(starts), n, tokens, max_q, max_kv,
+                       s.k_dim ** -0.5 if scale is None else scale, window, _ptr(sink),
+                       _ptr(workspace), workspace.nbytes, self._stream())
+        return out if lse is None else (out, lse)
 
     def expert_workspace_bytes(self, inter):
         self.lib.dsv4g_expert_workspace_bytes.restype = C.c_size_t
@@ -487,6 +720,70 @@ class DeviceLayer:
         meta = {k: layer[k] for k in ("hidden", "inter", "n_experts", "topk", "route_scale",
                                       "swiglu_limit", "expert_stride", "scale_run")}
         return cls(t, meta)
+
+
+CACHE_FULL, CACHE_LIST, CACHE_PAGE = 1, 2, 4  # DSV4G_CACHE_*: bits of the status word
+
+
+class PagedCache:
+    """A DSV4GCache over the caller's tensors, kept alive here: pages uint8
+    [n_layers][n_pages][page_bytes], ref int32 [n_pages], table int32
+    [n_seqs][max_pages], length int32 [n_seqs], status int32 [1]. dtype "bf16"
+    or "fp8"; v_dim 0: the values are the keys."""
+
+    def __init__(self, pages, ref, table, length, status, page_size, kv_heads, k_dim, v_dim=0,
+                 dtype="bf16"):
+        import torch
+        if dtype not in ("bf16", "fp8"):
+            raise ValueError(f"PagedCache: dtype {dtype!r}, 'bf16' or 'fp8' needed")
+        if pages.dim() != 3 or pages.dtype != torch.uint8 or not pages.is_contiguous():
+            raise ValueError("PagedCache: pages must be contiguous uint8 "
+                             "[n_layers][n_pages][page_bytes]")
+        if table.dim() != 2:
+            raise ValueError("PagedCache: table must be [n_seqs][max_pages]")
+        _same_device("PagedCache", pages, ref, table, length, status)
+        _int32("PagedCache", ref, pages.shape[1])
+        _int32("PagedCache", table, table.shape[0] * table.shape[1])
+        _int32("PagedCache", length, table.shape[0])
+        _int32("PagedCache", status, 1)
+        self.pages, self.ref, self.table, self.length = pages, ref, table, length
+        self.status, self.device = status, pages.device
+        s = self.struct = DSV4GCache()
+        for name, t in (("pages", pages), ("ref", ref), ("table", table), ("len", length),
+                        ("status", status)):
+            setattr(s, name, t.data_ptr())
+        s.n_layers, s.n_pages = pages.shape[:2]
+        s.page_size, s.kv_heads, s.k_dim, s.v_dim = page_size, kv_heads, k_dim, v_dim
+        s.dtype = DTYPE_CODES["F8_E4M3" if dtype == "fp8" else "BF16"]
+        s.n_seqs, s.max_pages = table.shape
+        need = self.page_bytes(s)
+        if need == 0 or pages.shape[2] != need:
+            raise ValueError(f"PagedCache: pages of {pages.shape[2]} bytes, this shape takes "
+                             f"{need or 'none (not a cache shape)'}")
+
+    @staticmethod
+    def page_bytes(struct):
+        return int(lib().lib.dsv4g_cache_page_bytes(C.byref(struct)))
+
+    @classmethod
+    def new(cls, n_layers, n_pages, page_size, kv_heads, k_dim, v_dim, n_seqs, max_pages,
+            dtype="bf16", device="cuda"):
+        """A cache of its own tensors, empty."""
+        import torch
+        s = DSV4GCache()
+        s.n_layers, s.n_pages, s.page_size, s.kv_heads = n_layers, n_pages, page_size, kv_heads
+        s.k_dim, s.v_dim, s.n_seqs, s.max_pages = k_dim, v_dim, n_seqs, max_pages
+        s.dtype = DTYPE_CODES["F8_E4M3" if dtype == "fp8" else "BF16"]
+        size = cls.page_bytes(s)
+        if size == 0:
+            raise ValueError("PagedCache: not a cache shape")
+        i = dict(dtype=torch.int32, device=device)
+        c = cls(torch.empty(n_layers, n_pages, size, dtype=torch.uint8, device=device),
+                torch.empty(n_pages, **i), torch.empty(n_seqs, max_pages, **i),
+                torch.empty(n_seqs, **i), torch.empty(1, **i), page_size, kv_heads, k_dim, v_dim,
+                dtype)
+        lib().cache_init(c)
+        return c
 
 
 class StTensor(C.Structure):

@@ -43,6 +43,10 @@ extern "C" {
 #define DSV4G_EINVAL 1 /* bad argument or unsupported shape */
 #define DSV4G_EHIP 2   /* HIP runtime error */
 
+/* Types of tensors, logits, activations and cache pages. */
+enum { DSV4G_DT_UNKNOWN = 0, DSV4G_DT_U8, DSV4G_DT_BF16, DSV4G_DT_F16, DSV4G_DT_F32,
+       DSV4G_DT_I8, DSV4G_DT_I64, DSV4G_DT_F8_E4M3, DSV4G_DT_F8_E8M0 };
+
 /* One MoE layer resident in HBM (device pointers). Routed expert e occupies
  * expert_stride bytes at experts + e*expert_stride: the E8M0 scale run
  * [w1 | w2 | w3] (per row, per 32 columns) followed at +scale_run by the
@@ -132,6 +136,29 @@ int dsv4g_gemv_bf16(float *y, const float *x, const uint16_t *W, int in, int out
  * 0 when logits[0] is NaN. idx [n], device. */
 int dsv4g_argmax(int *idx, const float *logits, int vocab, int n, size_t stride,
                  void *stream);
+/* Scores of given tokens under n rows of logits (F32 or BF16, dtype
+ * DSV4G_DT_F32 / _BF16; row r at logits + r * stride elements), with
+ * z = scale * logit in fp32 (scale > 0: 1 / temperature), lse = log sum e^z:
+ *   logprob[r]  z[token] - lse                  (tokens[r], or tokens NULL)
+ *   rank[r]     tokens with a larger z, or an equal one at a lower index (0:
+ *               the greedy token)
+ *   entropy[r]  lse - sum e^(z - lse) z
+ *   top_id, top_logprob [n][k], k <= DSV4G_MAX_TOP: the k largest z, the
+ *               lower index first where they are equal; their z - lse.
+ * Outputs may be NULL. A logit of -inf is a token that cannot be taken: it adds
+ * nothing. A token outside [0, vocab) gives a NaN logprob and rank -1; k above
+ * vocab leaves id -1 and NaN behind the vocab entries. A row whose largest
+ * logit is infinite, or that holds a NaN, has NaN log probabilities and
+ * entropy and rank -1 (among the top k a NaN logit counts as -inf). workspace: 256-byte aligned, at least
+ * dsv4g_logprobs_workspace_bytes(vocab, n, k) (0: none is needed, and it may
+ * be NULL); a call uses nothing that an earlier one left there. No
+ * counterpart in the reference. */
+#define DSV4G_MAX_TOP 64
+size_t dsv4g_logprobs_workspace_bytes(int vocab, int n, int k);
+int dsv4g_logprobs(float *logprob, float *entropy, int *rank, int *top_id, float *top_logprob,
+                   const void *logits, int dtype, int vocab, int n, size_t stride,
+                   const int *tokens, int k, float scale, void *workspace,
+                   size_t workspace_bytes, void *stream);
 /* dsv4_gemv_fp8 (mode 0) / dsv4_gemv_fp8_tbl (mode 1) (include/dsv4/dsv4.h:200-206)
  * and dsv4_gemv_fp4 (include/dsv4/dsv4.h:208-211), float block scales. */
 int dsv4g_gemv_fp8_float(float *y, const float *x, const uint8_t *W, const float *wscale,
@@ -339,6 +366,126 @@ int dsv4g_ffn_step(float *state, const float *hc_fn, const float *hc_scale,
                    float hc_eps, void *workspace, size_t workspace_bytes, int *idx_out,
                    float *wt_out, void *stream);
 
+/* ------------------------------------- paged cache and attention over it ----
+ * What a layer's attention half needs between its projections (wq_b, wkv ->
+ * wo_b): keys and values of several sequences in pages of one pool, and the
+ * attention of a chunk of new tokens per sequence over them. No counterpart
+ * in the reference, whose attention stays on the host.
+ *
+ * A page holds page_size tokens of one layer: keys
+ * [kv_heads][page_size][k_dim], then values [kv_heads][page_size][v_dim]
+ * (v_dim 0: the values are the keys, one latent row per token and head).
+ * DSV4G_DT_BF16: two bytes each. DSV4G_DT_F8_E4M3: one code each, then in the
+ * same order an E8M0 code per DSV4G_CACHE_GROUP columns
+ * ([kv_heads][page_size][k_dim / 64], the values' after them); a value is
+ * code * 2^(scale - 127). A page takes dsv4g_cache_page_bytes(C), a multiple
+ * of 256; page p of layer l is at pages + (l * n_pages + p) * that.
+ *
+ * Sequence s (a row of the table) holds len[s] tokens; its j-th token lies in
+ * page table[s][j / page_size]. Entries behind its pages are -1. ref[p] counts
+ * the table entries that name page p; 0: the page is free. Sequences share
+ * pages after a fork; a shared page is never written into
+ * (dsv4g_cache_reserve copies it first).
+ *
+ * Calls take a list of n_seqs sequences (seqs: device, NULL for 0 .. n_seqs -
+ * 1) and, where tokens go with them, starts (device, n_seqs + 1 entries): the
+ * new tokens of the i-th listed sequence are rows starts[i] ..
+ * starts[i + 1] - 1 of the call's token arrays, and they are the last ones of
+ * that sequence (positions len - count .. len - 1 once reserved). Rows at or
+ * behind starts[n_seqs] are left alone.
+ *
+ * What only the device knows is checked there: a list that names a sequence
+ * twice or out of range, a length or a table entry that cannot be. Such an
+ * entry is skipped (by dsv4g_cache_reserve: the whole call) and sets a bit of
+ * the sticky *status. While *status is not 0, dsv4g_cache_reserve, _append and
+ * dsv4g_attention do nothing (their outputs are left as they were), so that no
+ * later call of an engine's queue works on a cache that the refused call did
+ * not prepare. dsv4g_cache_status reads and clears it. Calls on one cache
+ * must be ordered (one stream, or events). */
+#define DSV4G_CACHE_GROUP 64
+#define DSV4G_CACHE_MAX_SEQS 1024 /* listed in one _reserve, _fork or _free */
+#define DSV4G_CACHE_FULL 1u       /* *status: fewer free pages than reserve needed */
+#define DSV4G_CACHE_LIST 2u       /* a listed sequence, count or length that cannot be */
+#define DSV4G_CACHE_PAGE 4u       /* a table entry that is no page */
+typedef struct {
+    uint8_t *pages;   /* device, 256-byte aligned: [n_layers][n_pages][page_bytes] */
+    int *ref;         /* device [n_pages] */
+    int *table;       /* device [n_seqs][max_pages] */
+    int *len;         /* device [n_seqs] */
+    unsigned *status; /* device, one word */
+    int n_layers, n_pages;
+    int page_size;    /* tokens: a power of two, 16 .. 256 */
+    int kv_heads;
+    int k_dim, v_dim; /* 64, 128 or 256 each and equal; or v_dim 0 and k_dim 256 or 512 */
+    int dtype;        /* DSV4G_DT_BF16 or DSV4G_DT_F8_E4M3 */
+    int n_seqs, max_pages;
+} DSV4GCache;
+size_t dsv4g_cache_page_bytes(const DSV4GCache *C); /* 0: not a valid shape */
+/* Every sequence empty, every page free, status 0 (the pages are not touched). */
+int dsv4g_cache_init(const DSV4GCache *C, void *stream);
+/* *status into *status_out (host) with a synchronisation, then cleared. */
+int dsv4g_cache_status(unsigned *status_out, const DSV4GCache *C, void *stream);
+/* Room for the new tokens: len grows by each listed count, with free pages
+ * (the lowest numbers first, in the order of the list) for what the last page
+ * does not hold, and a copy of its own of a last page that the sequence
+ * shares and would write into (every layer's; among listed sequences that
+ * share it, the first ones copy). All of the call or, with a status bit,
+ * nothing. workspace: 256-byte aligned, dsv4g_cache_workspace_bytes(C). */
+size_t dsv4g_cache_workspace_bytes(const DSV4GCache *C);
+int dsv4g_cache_reserve(const DSV4GCache *C, const int *seqs, const int *starts, int n_seqs,
+                        void *workspace, size_t workspace_bytes, void *stream);
+/* The new tokens' rows into the pages of one layer: k [n_tokens][kv_heads][k_dim]
+ * with k_stride elements from token to token, v likewise (NULL with v_dim 0),
+ * act_dtype DSV4G_DT_F32 or _BF16, 16-byte aligned rows. BF16 pages: rounded to
+ * nearest even. E4M3 pages: the scale is the power of two that the activation
+ * quantisation takes (2^ceil(log2(max(amax, 1e-4) / 448)), over the group's
+ * finite values), codes to nearest even; infinities are held as NaN. A
+ * sequence listed twice is not written. */
+int dsv4g_cache_append(const DSV4GCache *C, int layer, const void *k, size_t k_stride,
+                       const void *v, size_t v_stride, int act_dtype, const int *seqs,
+                       const int *starts, int n_seqs, int n_tokens, void *stream);
+/* Sequence children[i], which must be empty, becomes a copy of parents[i]: it
+ * holds the same pages. A parent may be listed more than once; a child listed
+ * twice, or as a parent too, is skipped with a status bit. */
+int dsv4g_cache_fork(const DSV4GCache *C, const int *parents, const int *children, int n_seqs,
+                     void *stream);
+/* The listed sequences cut back to new_len tokens (device; NULL: 0, the whole
+ * sequence): pages behind them lose a user, and are free at 0. */
+int dsv4g_cache_free(const DSV4GCache *C, const int *seqs, const int *new_len, int n_seqs,
+                     void *stream);
+/* Moves the pages in use to the front of the pool: with n of them, the i-th
+ * used page at or behind n goes to the i-th free one before n (every layer's
+ * contents, its ref, and the table entries that name it). n_used: device,
+ * optional. workspace as for reserve. */
+int dsv4g_cache_compact(const DSV4GCache *C, int *n_used, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* Attention of the new tokens of every listed sequence over the cache of one
+ * layer, which already holds them (reserve, then append): query head h of
+ * heads reads kv head h / (heads / kv_heads); the token at position p sees
+ * positions max(0, p - window + 1) .. p (window 0: all up to p);
+ *   out = sum_j e^(z_j) v_j / (sum_j e^(z_j) + e^(sink[h])), z_j = scale q.k_j,
+ * lse = log of the denominator. sink: F32 [heads] or NULL (no such term). A
+ * row that sees nothing has out 0 and lse -inf (or the sink). Tokens that a
+ * row does not see have no influence on it, whatever they hold.
+ * q [n_tokens][heads][k_dim] with q_stride elements from token to token, out
+ * [n_tokens][heads][v_dim or k_dim] with out_stride, both act_dtype:
+ * DSV4G_DT_BF16, or DSV4G_DT_F32 holding BF16 values as every activation here
+ * does (q is rounded to BF16, out is rounded to BF16); 16-byte aligned rows.
+ * lse: F32 [n_tokens][heads], optional. max_q, max_kv: host bounds of the
+ * listed counts and lengths (a sequence beyond them is skipped with a status
+ * bit); they size the launch. seqs may name a sequence more than once.
+ * workspace: 256-byte aligned, at least dsv4g_attention_workspace_bytes (0:
+ * none is needed, and it may be NULL); a call uses nothing that an earlier
+ * one left there. */
+size_t dsv4g_attention_workspace_bytes(const DSV4GCache *C, int heads, int n_seqs, int n_tokens,
+                                       int max_q, int max_kv);
+int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, size_t q_stride,
+                    int act_dtype, const DSV4GCache *C, int layer, int heads, const int *seqs,
+                    const int *starts, int n_seqs, int n_tokens, int max_q, int max_kv,
+                    float scale, int window, const float *sink, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------ checkpoint index + HBM loader
  * The safetensors index replaces the reference reader K3St
  * (src/io/k3_st.h:34-103): k3_st_open / close / find / read / read_f32 /
@@ -350,9 +497,6 @@ int dsv4g_ffn_step(float *state, const float *hc_fn, const float *hc_scale,
  * every expert resident in HBM there is no per-token streaming. Index calls
  * touch no GPU. Errors: DSV4G_EIO with the message in dsv4g_last_error(). */
 #define DSV4G_EIO 3 /* checkpoint file missing, malformed or short */
-
-enum { DSV4G_DT_UNKNOWN = 0, DSV4G_DT_U8, DSV4G_DT_BF16, DSV4G_DT_F16, DSV4G_DT_F32,
-       DSV4G_DT_I8, DSV4G_DT_I64, DSV4G_DT_F8_E4M3, DSV4G_DT_F8_E8M0 };
 
 typedef struct {
     const char *name;

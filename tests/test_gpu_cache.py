@@ -1,0 +1,284 @@
+"""The paged cache on the GPU against its definition (tests/paged.py): the
+bookkeeping as whole numbers, the pages' bytes as copies and as roundings of
+the appended rows."""
+import random
+
+import pytest
+
+import common  # noqa: F401  (the path of the binding)
+import paged
+from paged import FULL, LIST, PAGE, Book
+
+pytestmark = pytest.mark.gpu
+SHAPES = [(16, 1, 512, 0, True), (32, 2, 64, 64, False), (64, 3, 128, 128, True),
+          (256, 1, 256, 256, False), (128, 2, 256, 0, True)]
+
+
+@pytest.fixture(scope="module")
+def env():
+    import torch
+    import dsv4_gpu
+    return dict(torch=torch, lib=dsv4_gpu.lib(), gpu=dsv4_gpu, dev=torch.device("cuda:0"))
+
+
+def ints(env, v):
+    return env["torch"].tensor(list(v), dtype=env["torch"].int32, device=env["dev"])
+
+
+def starts_of(env, counts):
+    return ints(env, [sum(counts[:i]) for i in range(len(counts) + 1)])
+
+
+def new_cache(env, shape, layers=2, pages=40, seqs=9, cols=12):
+    ps, kvh, k, v, fp8 = shape
+    c = env["gpu"].PagedCache.new(layers, pages, ps, kvh, k, v, seqs, cols,
+                                  "fp8" if fp8 else "bf16", env["dev"])
+    g = env["torch"].Generator(device=env["dev"]).manual_seed(1)
+    c.pages.copy_(env["torch"].randint(0, 256, c.pages.shape, generator=g, device=env["dev"],
+                                       dtype=env["torch"].uint8))
+    return c, Book(pages, seqs, cols, ps)
+
+
+def check(env, c, book, image, status=True):
+    assert c.ref.tolist() == book.ref
+    assert c.length.tolist() == book.len
+    assert c.table.tolist() == book.table
+    if image is not None:
+        assert env["torch"].equal(c.pages, image)
+    if status:
+        assert env["lib"].cache_status(c) == book.status
+        book.status = 0
+
+
+def moved(image, moves):
+    out = image.clone()
+    for a, b in moves:
+        out[:, b] = image[:, a]
+    return out
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_random_bookkeeping(env, shape, seed):
+    """Two hundred calls drawn at random, refused ones among them, on a pool
+    that is often full; state and pages equal after each."""
+    lib, rng = env["lib"], random.Random(seed)
+    c, book = new_cache(env, shape)
+    n, ps = len(book.len), book.ps
+    image = c.pages.clone()
+    for step in range(120):
+        some = rng.sample(range(n), rng.randint(1, 5))
+        what = rng.random()
+        if what < 0.45:
+            counts = [rng.choice((0, 1, 5, ps, rng.randint(0, 3 * ps))) for _ in some]
+            if rng.random() < 0.05:
+                some[-1] = some[0] if len(some) > 1 else n
+            if rng.random() < 0.05:
+                counts[0] = 13 * ps
+            lib.cache_reserve(c, starts_of(env, counts), ints(env, some))
+            if any(x < 0 for x in counts):
+                continue
+            image = moved(image, book.reserve(some, counts))
+        elif what < 0.7:
+            parents = [rng.randrange(n) for _ in some]
+            lib.cache_fork(c, ints(env, parents), ints(env, some))
+            book.fork(parents, some)
+        elif what < 0.95:
+            to = [rng.choice((0, book.len[s], rng.randint(0, book.len[s]), book.len[s] + 1))
+                  if rng.random() < 0.3 else rng.randint(0, book.len[s]) for s in some]
+            whole = rng.random() < 0.2
+            lib.cache_free(c, ints(env, some), None if whole else ints(env, to))
+            book.free(some, [0] * len(some) if whole else to)
+        else:
+            used = ints(env, [-5])
+            lib.cache_compact(c, used)
+            image = moved(image, book.compact())
+            assert used.tolist() == [sum(r > 0 for r in book.ref)]
+        check(env, c, book, image)
+
+
+def test_copy_on_write_of_many(env):
+    """Four sequences that share a partly filled page all grow: three copy (the
+    first ones of the list), the last one keeps the page; contents equal."""
+    lib = env["lib"]
+    c, book = new_cache(env, SHAPES[0])
+    image = c.pages.clone()
+    for fn, a in ((lib.cache_reserve, ([20], [0])),):
+        fn(c, starts_of(env, a[0]), ints(env, a[1]))
+        book.reserve(a[1], a[0])
+    lib.cache_fork(c, ints(env, [0, 0, 0]), ints(env, [1, 2, 3]))
+    book.fork([0, 0, 0], [1, 2, 3])
+    lib.cache_reserve(c, starts_of(env, [1, 1, 1, 1]), ints(env, [3, 1, 0, 2]))
+    moves = book.reserve([3, 1, 0, 2], [1, 1, 1, 1])
+    assert len(moves) == 3
+    check(env, c, book, moved(image, moves))
+
+
+def test_full_pool_changes_nothing_and_blocks(env):
+    torch, lib = env["torch"], env["lib"]
+    c, book = new_cache(env, SHAPES[1], pages=6)
+    lib.cache_reserve(c, starts_of(env, [100]), ints(env, [0]))
+    book.reserve([0], [100])
+    check(env, c, book, None)
+    image = c.pages.clone()
+    lib.cache_reserve(c, starts_of(env, [10, 200]), ints(env, [0, 1]))
+    # blocked until the status is read: append, attention and another reserve
+    st = starts_of(env, [5])
+    k = torch.randn(5, 2, 64, device=env["dev"])
+    lib.cache_append(c, 0, k, k, st, ints(env, [0]))
+    lib.cache_reserve(c, st, ints(env, [0]))
+    out = torch.full((5, 4, 64), 7.0, dtype=torch.bfloat16, device=env["dev"])
+    lse = torch.full((5, 4), 7.0, device=env["dev"])
+    lib.attention(c, 0, out.clone(), st, ints(env, [0]), out=out, lse=lse)
+    assert (out == 7).all() and (lse == 7).all()
+    book.status = FULL
+    check(env, c, book, image)
+    lib.cache_reserve(c, st, ints(env, [0]))  # works again
+    book.reserve([0], [5])
+    check(env, c, book, image)
+
+
+def test_large_pool_and_table(env):
+    """More pages than one step of the scan, found near the end."""
+    torch, lib = env["torch"], env["lib"]
+    c, book = new_cache(env, (16, 1, 64, 64, True), layers=1, pages=20011, seqs=3, cols=20011)
+    lib.cache_reserve(c, starts_of(env, [16 * 20000]), ints(env, [1]))
+    book.reserve([1], [16 * 20000])
+    lib.cache_reserve(c, starts_of(env, [100, 3]), ints(env, [0, 2]))
+    book.reserve([0, 2], [100, 3])
+    lib.cache_free(c, ints(env, [1]), ints(env, [5000]))
+    book.free([1], [5000])
+    image = c.pages.clone()
+    check(env, c, book, image)
+    lib.cache_compact(c)
+    check(env, c, book, moved(image, book.compact()))
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+def test_append(env, shape, kind):
+    """Ragged counts with zeros, strided rows, rows in front of and behind the
+    listed ones, values that round, overflow the group's scale, NaN and
+    infinities; the other layer, slots and sequences stay as they were."""
+    torch, lib = env["torch"], env["lib"]
+    ps, kvh, kd, vd, fp8 = shape
+    c, book = new_cache(env, shape, cols=6)
+    g = torch.Generator(device=env["dev"]).manual_seed(3)
+    held, counts, seqs = [5, 0, ps, 2 * ps - 1], [7, 0, 1, ps + 3], [4, 1, 0, 7]
+    lib.cache_reserve(c, starts_of(env, held), ints(env, seqs))
+    lib.cache_reserve(c, starts_of(env, counts), ints(env, seqs))
+    book.reserve(seqs, held), book.reserve(seqs, counts)
+    front, rows = 2, sum(counts) + 2 + 3
+    starts = starts_of(env, counts) + front
+    dt = getattr(torch, kind)
+    wide = [torch.randn(rows, kvh * d + 16, generator=g, device=env["dev"]) * 3 for d in (kd, vd)]
+    for w in wide:
+        w[3] *= 1e-6       # below the scale's floor
+        w[4] *= 1e30
+        w[5, ::7] = 0
+        w[6, 3], w[6, 70 % w.shape[1]], w[6, 5] = float("nan"), float("inf"), float("-inf")
+    k, v = [w.to(dt)[:, :kvh * d].unflatten(1, (kvh, d)) if d else None
+            for w, d in zip(wide, (kd, vd))]
+    image = c.pages.clone()
+    lib.cache_append(c, 1, k, v, starts, ints(env, seqs))
+    check(env, c, book, None)
+    size, v_off, ks, vs = paged.page_layout(ps, kvh, kd, vd, fp8)
+    want = image.clone()
+    for new, d, at, sat in ((k, kd, 0, ks), (v, vd, v_off, vs)):
+        if new is None:
+            continue
+        x = new.float().cpu()
+        if fp8:
+            x = x.unflatten(-1, (-1, 64))
+            fin = torch.where(torch.isfinite(x), x.abs(), 0.0)
+            r = fin.amax(-1).clamp(min=1e-4) * torch.tensor(1 / 448)
+            bits = r.view(torch.int32)
+            code = (bits >> 23) + ((bits & 0x7FFFFF) != 0)
+            q = (x / (code << 23).view(torch.float32)[..., None])
+            byte = q.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+            byte = torch.where(torch.isfinite(x), byte, byte | 0x7F).flatten(-2)
+            code = code.to(torch.uint8)
+        else:
+            byte = x.to(torch.bfloat16).contiguous().view(torch.uint8)
+        u = 1 if fp8 else 2
+        for i, (s, n) in enumerate(zip(seqs, counts)):
+            for j in range(n):
+                row = int(starts[i]) + j
+                pos = held[i] + j
+                page, slot = book.table[s][pos // ps], pos % ps
+                for h in range(kvh):
+                    e = (h * ps + slot) * d
+                    want[1, page, at + u * e:at + u * (e + d)] = byte[row, h].to(env["dev"])
+                    if fp8:
+                        want[1, page, sat + e // 64:sat + (e + d) // 64] = \
+                            code[row, h].to(env["dev"])
+    if not fp8:  # a NaN is a NaN, whatever its bits
+        a, b = c.pages.view(torch.bfloat16), want.view(torch.bfloat16)
+        same = (a.view(torch.int16) == b.view(torch.int16)) | (a.isnan() & b.isnan())
+    else:
+        same = c.pages == want
+        nan = ((c.pages & 0x7F) == 0x7F) & ((want & 0x7F) == 0x7F)
+        same |= nan
+    assert same.all(), (~same).nonzero()[:5]
+
+
+def test_append_refuses_on_device(env):
+    """A sequence listed twice, one out of range, more new tokens than the
+    sequence holds, a table entry that is no page: not written, a status bit."""
+    torch, lib = env["torch"], env["lib"]
+    c, book = new_cache(env, SHAPES[1])
+    lib.cache_reserve(c, starts_of(env, [40, 40, 40]), ints(env, [0, 1, 2]))
+    book.reserve([0, 1, 2], [40, 40, 40])
+    check(env, c, book, None)
+    k = torch.randn(6, 2, 64, device=env["dev"])
+    for seqs, counts, bit in (([0, 0], [2, 2], LIST), ([1, 9], [0, 3], LIST),
+                              ([-1], [3], LIST), ([2], [41], LIST), ([3], [1], LIST)):
+        image = c.pages.clone()
+        big = torch.randn(sum(counts), 2, 64, device=env["dev"])
+        lib.cache_append(c, 0, big, big, starts_of(env, counts), ints(env, seqs))
+        assert lib.cache_status(c) == bit, seqs
+        if len(seqs) == 1 and counts[0] <= 40:
+            assert torch.equal(c.pages, image)
+    for entry in (-1, 40, 2 ** 31 - 1, -2 ** 31):
+        c.table[1, 1] = entry
+        image = c.pages.clone()
+        lib.cache_append(c, 0, k, k, starts_of(env, [6]), ints(env, [1]))
+        assert lib.cache_status(c) == PAGE
+        assert torch.equal(c.pages, image)
+
+
+def test_bookkeeping_in_a_graph(env):
+    """A captured fork - reserve - free of the child, replayed with eager work
+    between: every replay leaves what the eager calls leave."""
+    torch, lib = env["torch"], env["lib"]
+    c, book = new_cache(env, SHAPES[2])
+    lib.cache_reserve(c, starts_of(env, [70, 9]), ints(env, [0, 1]))
+    book.reserve([0, 1], [70, 9])
+    ws = torch.empty(lib.cache_workspace_bytes(c), dtype=torch.uint8, device=env["dev"])
+    kids, olds, st = ints(env, [5, 6]), ints(env, [0, 1]), starts_of(env, [4, 60])
+    back = ints(env, [72, 9])
+
+    def step():
+        lib.cache_fork(c, olds, kids)
+        lib.cache_reserve(c, st, kids, workspace=ws)
+        lib.cache_free(c, kids, back)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        lib.cache_free(c, kids)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    book.fork([0, 1], [5, 6])
+    moves = book.reserve([5, 6], [4, 60])
+    book.free([5, 6], [72, 9])
+    for i in range(4):
+        image = c.pages.clone()
+        graph.replay()
+        check(env, c, book, moved(image, moves))
+        lib.cache_free(c, kids)
+        (c.pages.float().sum() * i).item()
