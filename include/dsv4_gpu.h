@@ -465,14 +465,16 @@ int dsv4g_cache_compact(const DSV4GCache *C, int *n_used, void *workspace,
  * heads reads kv head h / (heads / kv_heads); the token at position p sees
  * positions max(0, p - window + 1) .. p (window 0: all up to p);
  *   out = sum_j e^(z_j) v_j / (sum_j e^(z_j) + e^(sink[h])), z_j = scale q.k_j,
- * lse = log of the denominator. sink: F32 [heads] or NULL (no such term). A
- * row that sees nothing has out 0 and lse -inf (or the sink). Tokens that a
- * row does not see have no influence on it, whatever they hold.
+ * lse = log of the denominator. sink: F32 [heads] or NULL (no such term).
+ * Tokens that a row does not see have no influence on it, whatever they hold;
+ * a row that sees a key or value that is not finite is not finite in the
+ * columns concerned (which others are not is left open).
  * q [n_tokens][heads][k_dim] with q_stride elements from token to token, out
  * [n_tokens][heads][v_dim or k_dim] with out_stride, both act_dtype:
  * DSV4G_DT_BF16, or DSV4G_DT_F32 holding BF16 values as every activation here
  * does (q is rounded to BF16, out is rounded to BF16); 16-byte aligned rows.
- * lse: F32 [n_tokens][heads], optional. max_q, max_kv: host bounds of the
+ * lse: F32 [n_tokens][heads], optional. The outputs of a call that sets a
+ * status bit are not valid. max_q, max_kv: host bounds of the
  * listed counts and lengths (a sequence beyond them is skipped with a status
  * bit); they size the launch. seqs may name a sequence more than once.
  * workspace: 256-byte aligned, at least dsv4g_attention_workspace_bytes (0:
