@@ -33,10 +33,12 @@ typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
 typedef float F16v __attribute__((ext_vector_type(16)));
 typedef short S4 __attribute__((ext_vector_type(4)));
 typedef int I4 __attribute__((ext_vector_type(4)));
+typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+// LDS by address
+#define DSV4_LDS(T, at) (*(__attribute__((address_space(3))) T *)(uintptr_t)(at))
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float AT_GROW = 8.0f;  // log2 of what the weights may grow to before a rescaling
-constexpr int AT_MAX_SPLIT = 64;
 
 struct AttnArgs {
   void *out;
@@ -45,30 +47,45 @@ struct AttnArgs {
   size_t out_stride, q_stride;
   const int *seqs, *starts;
   const float *sink;
-  float *part;   // [item][split][ROWS * D] outputs not yet divided, in the waves' layout
-  float2 *stat;  // [item][split][ROWS] (m, l)
+  // shared work only: outputs not yet divided [workgroup][2][ROWS * D] in the
+  // waves' layout, their rows' (m, l) [workgroup][2][ROWS], the position of
+  // each item's first stage, and the number of all stages
+  float *part;
+  float2 *stat;
+  long *first;
   int layer, heads, group, n_seqs, n_tokens, max_q, max_kv, window, f32;
-  int tiles, nsplit, items;
+  int tiles, groups;  // groups: workgroups that share the stages, or 0: one per item
   float scale;
 };
 
 // Row waves RW (32 rows each) and, with fewer than 4, KW = 4 / RW waves that
 // share a stage's tokens.
+constexpr int at_max(int a, int b) { return a > b ? a : b; }
+constexpr int at_min(int a, int b) { return a < b ? a : b; }
 template <int D, bool SHARED, bool FP8, int RW>
 struct Cfg {
   static constexpr int KW = 4 / RW, TT = 32 * KW, ROWS = 32 * RW;
-  static constexpr int ROWB = 2 * D, CH = D / 8;  // bytes and 16-byte chunks of a row
-  static constexpr int KB = TT * ROWB, STAGE = SHARED ? KB : 2 * KB;
-  // bytes of LDS: two workgroups per CU for narrow heads, all for wide ones
-  static constexpr int CAP = D <= 128 && RW > 1 ? 66 * 1024 : 132 * 1024;
-  static constexpr int FIT = CAP / STAGE;
-  static constexpr int NBUF = FP8 ? 2 : FIT > 4 ? 4 : FIT;
-  static constexpr bool OK = FIT >= 2;
   static constexpr int NP = D / 32;  // output tiles
+  static constexpr int KB = TT * 2 * D, M = SHARED ? 1 : 2, STAGE = KB * M;  // BF16 rows
+  // E4M3: codes, then scale codes, as they lie in the page
+  static constexpr int CODES = TT * D, SCALES = TT * D / 64, RAW = M * (CODES + SCALES);
+  // LDS: all of it for one workgroup per CU where the accumulators take the
+  // registers (D >= 256) or a stage is long, else half
+  static constexpr int CAP = (D <= 128 && (RW > 1 || (FP8 && D == 64)) ? 68 : 134) * 1024;
+  static constexpr bool OK = 2 * STAGE <= CAP || (FP8 && STAGE + 2 * RAW <= CAP);
+  // E4M3: two BF16 stages (the next one is converted while this one is
+  // multiplied) where three stages of codes still fit beside them
+  static constexpr bool TWICE = FP8 && 2 * STAGE + 3 * RAW <= CAP;
+  static constexpr int NTILE = FP8 ? (TWICE ? 2 : 1) : at_min(4, CAP / STAGE);
+  static constexpr int NRAW = FP8 ? at_min(4, (CAP - NTILE * STAGE) / RAW) : 0;
+  static constexpr int RING = FP8 ? NRAW : NTILE;  // stages that direct loads fill
+  // direct loads per wave and stage
+  static constexpr int PER = FP8 ? M * (at_max(1, CODES / 4096) + at_max(1, TT / 64))
+                                 : STAGE / 4096;
   // a wave's outputs and its rows' (m, l), handed over when waves share rows
   static constexpr int PART = 32 * D * 4 + 64 * 8, JOIN = KW > 1 ? RW * PART : 0;
-  static constexpr int LDS = NBUF * STAGE > JOIN ? NBUF * STAGE : JOIN;
-  static constexpr int WGS = D <= 128 && LDS <= 80 * 1024 ? 2 : 1;  // per CU
+  static constexpr int LDS = at_max(NTILE * STAGE + NRAW * RAW, JOIN);
+  static constexpr int WGS = LDS <= 80 * 1024 && D <= 128 ? 2 : 1;  // per CU
 };
 
 template <int D>
@@ -85,53 +102,130 @@ __device__ __forceinline__ constexpr int dim_of(int dt, int half) {
   return D >= 128 ? 16 * (8 * (dt / 4) + dt % 4 + 4 * half) : 16 * (dt + 2 * half);
 }
 
-// What a workgroup works on; false: nothing. Uniform.
+// One item: a tile of a sequence's rows of one kv head. Uniform.
 struct Item {
-  int b, kvh, tile, split, seq, start, count, len, r0, nrows, lo, hi, clear, s0, s1, parts;
+  int b, kvh, seq, start, count, len, r0, nrows, lo, hi, clear, stages;
 };
+// Rows tile * ROWS .. of the b-th listed sequence; false: there are none.
 template <int ROWS, int TT>
-__device__ __forceinline__ bool attn_item(const DSV4GCache &C, const AttnArgs &a, int id,
+__device__ __forceinline__ bool attn_item(const DSV4GCache &C, const AttnArgs &a, int b, int tile,
                                           Item &it) {
-  it.split = id % a.nsplit;
-  id /= a.nsplit;
-  it.kvh = id % C.kv_heads;
-  id /= C.kv_heads;
-  it.b = id % a.n_seqs;
-  it.tile = a.tiles - 1 - id / a.n_seqs;  // the longest ranges first
-  it.seq = a.seqs ? a.seqs[it.b] : it.b;
-  it.start = a.starts[it.b];
-  const long end = a.starts[it.b + 1];
+  it.b = b;
+  it.seq = a.seqs ? a.seqs[b] : b;
+  it.start = a.starts[b];
+  const long end = a.starts[b + 1];
   const long count = end - it.start;
   it.len = it.seq >= 0 && it.seq < C.n_seqs ? C.len[it.seq] : -1;
   if (it.start < 0 || end > a.n_tokens || count < 0 || count > a.max_q || it.len < count ||
       it.len > a.max_kv || it.len > (long)C.max_pages * C.page_size) {
-    if (it.tile == 0 && it.split == 0 && threadIdx.x == 0)
-      atomicOr(C.status, DSV4G_CACHE_LIST);
+    if (tile == 0) atomicOr(C.status, DSV4G_CACHE_LIST);
     return false;
   }
   it.count = (int)count;
-  it.r0 = it.tile * ROWS;
+  it.r0 = tile * ROWS;
   it.nrows = it.count * a.group;
   if (it.r0 >= it.nrows) return false;
   const int first = it.len - it.count + it.r0 / a.group;
   it.hi = it.len - it.count + (min(it.r0 + ROWS, it.nrows) - 1) / a.group + 1;
   it.clear = a.window ? max(0, first - a.window + 1) : 0;  // the first token that is seen
   it.lo = it.clear & ~31;
-  const int stages = (it.hi - it.lo + TT - 1) / TT;
-  const int per = (stages + a.nsplit - 1) / a.nsplit;
-  it.parts = (stages + per - 1) / per;
-  it.s0 = it.split * per;
-  it.s1 = min(stages, it.s0 + per);
+  it.stages = (it.hi - it.lo + TT - 1) / TT;
   return true;
 }
 
-// The page of the 16-token group that begins at token t, or -1.
-__device__ __forceinline__ int page_of(const DSV4GCache &C, const CacheGeom &G, const Item &it,
-                                       int t) {
-  if (t >= it.hi || t + 15 < it.clear) return -1;
-  const int *cell = C.table + (size_t)it.seq * C.max_pages + (t >> G.shift);
-  return *(const __attribute__((address_space(4))) int *)cell;  // written by earlier kernels only
+// Shared work (fewer items than the chip has places for): the stages of all
+// items in a row, items ordered by (sequence, tile), then kv head, are dealt
+// out in equal runs, so that long and short sequences fill every workgroup
+// alike. Workgroup w takes stages [w T / W, (w + 1) T / W).
+__device__ __forceinline__ int shared_groups(const AttnArgs &a, long total) {
+  return (int)(total < a.groups ? total : a.groups);
 }
+__device__ __forceinline__ long share_begin(long total, int groups, int w) {
+  return total * w / groups;
+}
+__device__ __forceinline__ int share_of(long total, int groups, long at) {
+  return (int)(((at + 1) * groups - 1) / total);
+}
+
+// Where this workgroup's run begins: every thread counts the stages of some
+// (sequence, tile) pairs, one of them finds the place.
+struct Place {
+  long at, end, total;
+  int pair, kvh, stage;
+};
+template <int ROWS, int TT>
+__device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &a, Place &p) {
+  __shared__ long s_sum[4];
+  __shared__ int s_at[3];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int pairs = a.n_seqs * a.tiles, per = (pairs + 255) / 256;
+  const int j0 = min(pairs, tid * per), j1 = min(pairs, j0 + per);
+  long mine = 0;
+  Item it;
+  for (int j = j0; j < j1; ++j)
+    if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, it)) mine += it.stages;
+  long x = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) s_sum[wave] = x;
+  __syncthreads();
+  long before = x - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    before += w < wave ? s_sum[w] : 0;
+    total += s_sum[w];
+  }
+  before *= C.kv_heads;
+  p.total = total * C.kv_heads;
+  const int groups = shared_groups(a, p.total);
+  p.at = p.end = 0;
+  if ((int)blockIdx.x >= groups) return;
+  p.at = share_begin(p.total, groups, blockIdx.x);
+  p.end = share_begin(p.total, groups, blockIdx.x + 1);
+  if (p.at >= before && p.at < before + mine * C.kv_heads)
+    for (int j = j0; j < j1; ++j)
+      if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, it)) {
+        const long all = (long)it.stages * C.kv_heads;
+        if (p.at < before + all) {
+          s_at[0] = j;
+          s_at[1] = (int)((p.at - before) / it.stages);
+          s_at[2] = (int)((p.at - before) % it.stages);
+          break;
+        }
+        before += all;
+      }
+  __syncthreads();
+  p.pair = __builtin_amdgcn_readfirstlane(s_at[0]);
+  p.kvh = __builtin_amdgcn_readfirstlane(s_at[1]);
+  p.stage = __builtin_amdgcn_readfirstlane(s_at[2]);
+}
+
+// A value whose uses are computed again each time: addresses derived from it
+// would else be kept in registers around the loop over the stages.
+__device__ __forceinline__ void fresh(int &x) { asm volatile("" : "+v"(x)); }
+
+// Direct loads to LDS, 16 or 4 bytes per lane (lane l's at `to` + its size *
+// l). In inline asm: they have no output register, and the compiler would make
+// every later LDS read wait for all of them; wait_loads() and the barrier
+// order them instead.
+__device__ __forceinline__ void lds_load16(uint32_t to, uint32_t at, I4 rsrc) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               ::"s"(to), "v"(at), "s"(rsrc)
+               : "memory");
+}
+__device__ __forceinline__ void lds_load4(uint32_t to, uint32_t at, I4 rsrc) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               ::"s"(to), "v"(at), "s"(rsrc)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 __device__ __forceinline__ I4 page_rsrc(const DSV4GCache &C, const CacheGeom &G, int layer,
                                         int page) {
   const bool ok = page >= 0 && page < C.n_pages;
@@ -141,108 +235,153 @@ __device__ __forceinline__ I4 page_rsrc(const DSV4GCache &C, const CacheGeom &G,
   return I4{(int)(uint32_t)p, (int)(uint32_t)(p >> 32), ok ? (int)G.page_bytes : 0, 0x00020000};
 }
 
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-// BF16 pages: one stage's rows into LDS by direct loads (16 bytes per lane, 1
-// KB per instruction). Each wave brings TT / 4 tokens. In inline asm: a direct
-// load has no output register, and the compiler would make every later LDS
-// read wait for all of them; wait_loads() and the barrier order them instead.
-template <int D, bool SHARED, int TT>
-__device__ __forceinline__ void stage_bf16(const DSV4GCache &C, const CacheGeom &G,
-                                           const AttnArgs &a, const Item &it, const int (&page)[2],
-                                           int st, uint32_t lds, int wave, int lane) {
-  constexpr int CH = D / 8, TB = 64 / CH, TW = TT / 4, TG = TW < 16 ? TW : 16;
+// Brings stages of an item to LDS. Each wave brings a quarter of the tokens in
+// one or two groups of at most 16 (one page each); the pages of a stage are
+// looked up while the one before it is issued.
+constexpr uint32_t AT_OUT = 0x7FFFFFFFu;  // an offset behind any page: zeros
+template <int D, bool SHARED, bool FP8, int RW>
+struct Loader {
+  typedef Cfg<D, SHARED, FP8, RW> F;
+  // tokens of a wave's group, groups: E4M3 with narrow heads needs 16 tokens
+  // for one load, which the waves then bring twice
+  static constexpr int TT = F::TT, TW = TT / 4;
+  static constexpr int TG = FP8 ? (1024 / D > TW ? 1024 / D : at_min(16, TW)) : at_min(16, TW);
+  static constexpr int NG = at_max(1, TW / TG);
+  int page[NG];
+  __device__ __forceinline__ int first(int wave, int g) const {
+    return (wave * NG + g) * TG % TT;  // the stage's token where group g begins
+  }
+  __device__ __forceinline__ bool needed(const Item &it, int t) const {
+    return t < it.hi && t + TG > it.clear;
+  }
+  __device__ __forceinline__ void look(const DSV4GCache &C, const CacheGeom &G, const Item &it,
+                                       int st, int wave) {
 #pragma unroll
-  for (int g = 0; g < TW / TG; ++g) {
-    const int tl0 = wave * TW + g * TG;              // token of the stage
-    const int t0 = it.lo + st * TT + tl0;            // token of the sequence
-    const I4 rsrc = page_rsrc(C, G, a.layer, page[g]);
-    const int slot = t0 & (C.page_size - 1);
-    const uint32_t base = (uint32_t)((it.kvh * C.page_size + slot) * D * 2);
-#pragma unroll
-    for (int j = 0; j < TG / TB; ++j) {
-      const int off = j * TB + lane / CH;
-      uint32_t v = base + off * (2 * D) +
-                   16u * ((lane % CH) ^ chunk_swizzle<D>(tl0 + off));
-      const bool in = t0 + off < it.hi && t0 + off >= it.clear;
-      v = in ? v : 0x7FFFFFFFu;                      // zeros
-      const uint32_t to = lds + (tl0 + j * TB) * (2 * D);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   ::"s"(to), "v"(v), "s"(rsrc)
-                   : "memory");
-      if (!SHARED) {
-        const uint32_t vv = in ? v + G.v_off : 0x7FFFFFFFu;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                     ::"s"(to + TT * 2 * D), "v"(vv), "s"(rsrc)
-                     : "memory");
+    for (int g = 0; g < NG; ++g) {
+      const int t = it.lo + st * TT + first(wave, g);
+      page[g] = -1;
+      if (needed(it, t)) {
+        const int *cell = C.table + (size_t)it.seq * C.max_pages + (t >> G.shift);
+        // written by earlier kernels only
+        page[g] = *(const __attribute__((address_space(4))) int *)cell;
       }
     }
   }
-}
-
-// E4M3 pages: a stage's codes and scales into registers (16 codes per lane
-// and piece), and from there as BF16 into LDS. A code times its power of two
-// is exact in BF16. In two halves (where there are two pieces or more), one
-// under each product, so that half the registers hold loads in flight.
-template <int D, bool SHARED, int TT>
-struct Codes {
-  static constexpr int ALL = (TT * D + 4095) / 4096, M = SHARED ? 1 : 2;
-  static constexpr bool PART = TT * D < 4096;  // the stage takes the first waves only
-  static constexpr int H = ALL > 1 ? 2 : 1, N = ALL / H;  // halves, pieces of one
-  uint4 c[M][N];
-  uint32_t s[M][N];
-  __device__ __forceinline__ void load(const DSV4GCache &C, const CacheGeom &G, const AttnArgs &a,
-                                       const Item &it, int st, int half, int wave, int lane) {
-    if (PART && wave * 64 * 16 >= TT * D) return;
+  __device__ __forceinline__ void issue(const DSV4GCache &C, const CacheGeom &G, const AttnArgs &a,
+                                        const Item &it, int st, uint32_t lds, int wave, int lane) {
+    fresh(lane);
 #pragma unroll
-    for (int p = 0; p < N; ++p) {
-      // at most 16 tokens from here, one page
-      const int tl0 = ((half * N + p) * 256 + wave * 64) * 16 / D;
-      const int t0 = it.lo + st * TT + tl0;
-      const int page = page_of(C, G, it, t0);
-      const I4 r = page_rsrc(C, G, a.layer, page);
-      const BufRsrc rsrc = buf_rsrc((const void *)(((uint64_t)(uint32_t)r[1] << 32) |
-                                                   (uint32_t)r[0]), r[2]);
-      const int off = lane * 16 / D, col = lane * 16 % D;
-      const int slot = (t0 & (C.page_size - 1)) + off;
-      const uint32_t e = (uint32_t)(it.kvh * C.page_size + slot) * D + col;
-      const bool in = t0 + off < it.hi && t0 + off >= it.clear;
+    for (int g = 0; g < NG; ++g) {
+      const int tl0 = first(wave, g);
+      const int t0 = it.lo + st * TT + tl0;  // token of the sequence
+      if (needed(it, t0) && (page[g] < 0 || page[g] >= C.n_pages) && lane == 0)
+        atomicOr(C.status, DSV4G_CACHE_PAGE);
+      const I4 rsrc = page_rsrc(C, G, a.layer, page[g]);
+      const int slot = it.kvh * C.page_size + (t0 & (C.page_size - 1));
+      auto in = [&](int off) { return t0 + off < it.hi && t0 + off >= it.clear; };
+      if (!FP8) {
+        constexpr int CH = D / 8, TB = 64 / CH;  // chunks of a row, tokens per load
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        c[m][p] = buf_load16(rsrc, in ? e + (m ? G.v_off : 0) : 0x7FFFFFFFu);
-        s[m][p] = __builtin_amdgcn_raw_buffer_load_b8(
-            rsrc, in ? e / DSV4G_CACHE_GROUP + (m ? G.vs_off : G.ks_off) : 0x7FFFFFFFu, 0, 0);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(uint8_t *lds, int half, int wave, int lane) const {
-    if (PART && wave * 64 * 16 >= TT * D) return;
-#pragma unroll
-    for (int p = 0; p < N; ++p) {
-      const int tl = ((half * N + p) * 256 + wave * 64 + lane) * 16 / D, ch = lane * 16 % D / 8;
-      const int g = chunk_swizzle<D>(tl);
-#pragma unroll
-      for (int m = 0; m < M; ++m) {
-        const float scale = e8m0(s[m][p]);
-        const uint32_t u[4] = {c[m][p].x, c[m][p].y, c[m][p].z, c[m][p].w};
-        uint32_t y[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          y[2 * k] = __builtin_bit_cast(
-              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[k], scale, false));
-          y[2 * k + 1] = __builtin_bit_cast(
-              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[k], scale, true));
+        for (int j = 0; j < TG / TB; ++j) {
+          const int off = j * TB + lane / CH;
+          const uint32_t v = (uint32_t)(slot + off) * (2 * D) +
+                             16u * ((lane % CH) ^ chunk_swizzle<D>(tl0 + off));
+          const uint32_t to = lds + (tl0 + j * TB) * (2 * D);
+          lds_load16(to, in(off) ? v : AT_OUT, rsrc);
+          if (!SHARED) lds_load16(to + F::KB, in(off) ? v + G.v_off : AT_OUT, rsrc);
         }
-        uint8_t *row = lds + m * (TT * 2 * D) + tl * (2 * D);
-        *(uint4 *)(row + 16 * (ch ^ g)) = make_uint4(y[0], y[1], y[2], y[3]);
-        *(uint4 *)(row + 16 * ((ch + 1) ^ g)) = make_uint4(y[4], y[5], y[6], y[7]);
+      } else {
+        constexpr int TB = 1024 / D;  // tokens per load
+#pragma unroll
+        for (int j = 0; j < TG / TB; ++j) {
+          const int off = j * TB + lane * 16 / D;
+          const uint32_t v = (uint32_t)(slot + off) * D + lane * 16 % D;
+          const uint32_t to = lds + (tl0 + j * TB) * D;
+          lds_load16(to, in(off) ? v : AT_OUT, rsrc);
+          if (!SHARED) lds_load16(to + F::CODES + F::SCALES, in(off) ? v + G.v_off : AT_OUT, rsrc);
+        }
+      }
+    }
+    if (FP8) scales(C, G, a, it, st, lds, wave, lane);
+  }
+  // Scale codes, 16 tokens per load (4 bytes per lane): their group g16 has a
+  // page of its own lookup where the wave's codes lie in another page.
+  __device__ __forceinline__ void scales(const DSV4GCache &C, const CacheGeom &G,
+                                         const AttnArgs &a, const Item &it, int st, uint32_t lds,
+                                         int wave, int lane) {
+    constexpr int N = at_max(1, TT / 64), L = 4 * (D / 64);  // loads per wave, lanes of one
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int tl0 = (wave * N + k) * 16 % TT;
+      const int t0 = it.lo + st * TT + tl0;
+      int pg = -1;
+      if (t0 < it.hi && t0 + 16 > it.clear) {
+        const int *cell = C.table + (size_t)it.seq * C.max_pages + (t0 >> G.shift);
+        pg = *(const __attribute__((address_space(4))) int *)cell;
+      }
+      const I4 rsrc = page_rsrc(C, G, a.layer, pg);
+      const int slot = it.kvh * C.page_size + (t0 & (C.page_size - 1));
+      const int off = 4 * lane / (D / 64);  // token of this lane's first code
+      const bool some = t0 + off < it.hi && t0 + off + (D < 256 ? 256 / D : 1) > it.clear;
+      const uint32_t v = some ? (uint32_t)slot * (D / 64) + 4 * lane : AT_OUT;
+      const uint32_t to = lds + F::CODES + tl0 * (D / 64);
+      if (lane < L) {
+        lds_load4(to, some ? v + G.ks_off : AT_OUT, rsrc);
+        if (!SHARED) lds_load4(to + F::CODES + F::SCALES, some ? v + G.vs_off : AT_OUT, rsrc);
       }
     }
   }
 };
+
+// E4M3 codes of a stage as BF16 rows: a code times its power of two is exact
+// in BF16. 16 codes per thread and step.
+template <int D, bool SHARED, int TT>
+__device__ __forceinline__ void convert(uint32_t raw, uint32_t tile, int tid) {
+  constexpr int CODES = TT * D, SCALES = CODES / 64, KB = 2 * CODES;
+  fresh(tid);
+#pragma unroll
+  for (int m = 0; m < (SHARED ? 1 : 2); ++m) {
+    // a batch's reads at once and no branch: each step would else wait for LDS
+    constexpr int P = (CODES + 4095) / 4096, B = P < 4 ? P : 4;
+#pragma unroll
+    for (int p = 0; p < P; p += B) {
+      U4 u[B];
+      uint32_t s[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int at = ((p + i) * 256 + tid) * 16 % CODES;  // twice the same where there are fewer
+        u[i] = DSV4_LDS(U4, raw + at);
+        s[i] = DSV4_LDS(uint8_t, raw + CODES + at / 64);
+      }
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int at = ((p + i) * 256 + tid) * 16 % CODES;
+        const int tl = at / D, ch = at % D / 8, g = chunk_swizzle<D>(tl);
+        // E8M0; codes that were not loaded are 0, beside whatever scale the
+        // page holds
+        uint32_t bits = s[i] << 23;
+        bits = s[i] == 0 ? 0x00400000u : bits;
+        bits = s[i] == 255 ? 0x7FC00000u : bits;
+        bits = (u[i][0] | u[i][1] | u[i][2] | u[i][3]) == 0u ? 0x3F800000u : bits;
+        const float scale = u2f(bits);
+        U4 y[2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          y[k / 2][2 * (k % 2)] = __builtin_bit_cast(
+              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[i][k], scale, false));
+          y[k / 2][2 * (k % 2) + 1] = __builtin_bit_cast(
+              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[i][k], scale, true));
+        }
+        const uint32_t row = tile + tl * (2 * D);
+        DSV4_LDS(U4, row + 16 * (ch ^ g)) = y[0];
+        DSV4_LDS(U4, row + 16 * ((ch + 1) ^ g)) = y[1];
+      }
+      __builtin_amdgcn_sched_barrier(0);  // a batch at a time: registers
+    }
+    raw += CODES + SCALES;
+    tile += KB;
+  }
+}
 
 __device__ __forceinline__ float swap_max(float v) {  // with the other half of the wave
   const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
@@ -256,9 +395,6 @@ __device__ __forceinline__ float swap_sum(float v) {
 // LDS addresses. Rows are multiples of 128 bytes (256 where D >= 128), so the
 // chunk's XOR acts on address bits that hold nothing else, and every read is
 // the lane's one address XOR a constant plus a constant.
-typedef uint32_t U4 __attribute__((ext_vector_type(4)));
-#define DSV4_LDS(T, at) (*(__attribute__((address_space(3))) T *)(uintptr_t)(at))
-
 // First product: row lane % 32, columns 16 s + 8 h .. + 7.
 template <int D>
 __device__ __forceinline__ uint32_t k_at(int lane) {
@@ -296,6 +432,20 @@ __device__ __forceinline__ Bf8 read_vt(uint32_t at, int u, int dt) {
     r[2 * v + 1] = t.y;
   }
   return __builtin_bit_cast(Bf8, r);
+}
+
+// The order of a product's loop for the scheduler, which else puts each read
+// right in front of the product that waits for it: the LDS reads of the first
+// R steps, then a step's products and the reads of the step R on, in turn.
+constexpr int AT_AHEAD = 6;
+template <int N, int R, int MFMA, int READS>
+__device__ __forceinline__ void sched_steps() {
+  __builtin_amdgcn_sched_group_barrier(0x100, (R < N ? R : N) * READS, 0);
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    __builtin_amdgcn_sched_group_barrier(0x008, MFMA, 0);
+    if (s + R < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
 }
 
 // An output tile moved between the accumulation registers, where it stays in
@@ -353,305 +503,346 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
                                                                             CacheGeom G,
                                                                             AttnArgs a) {
   typedef Cfg<D, SHARED, FP8, RW> F;
-  constexpr int TT = F::TT, STAGE = F::STAGE, NBUF = F::NBUF, NP = F::NP, KS = D / 16;
+  constexpr int TT = F::TT, STAGE = F::STAGE, RING = F::RING, NP = F::NP, KS = D / 16;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[F::LDS];
   __shared__ uint32_t s_odd[F::KW];  // tokens of a stage with something not finite
   if (*C.status) return;
-  Item it;
-  if (!attn_item<F::ROWS, TT>(C, a, blockIdx.x, it) || it.s0 >= it.s1) return;
-  if (threadIdx.x < F::KW) s_odd[threadIdx.x] = 0;
   const int tid = threadIdx.x, lane = tid % 64, h = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int rw = wave % RW, kw = wave / RW;
-  // this lane's row (the last one again where there are fewer)
-  const int wr0 = it.r0 + 32 * rw;
-  const bool active = wr0 < it.nrows;
-  const int r = min(wr0 + lane % 32, it.nrows - 1);
-  const int tok = r / a.group, head = it.kvh * a.group + r % a.group;
-  const int pos0 = it.len - it.count, pos = pos0 + tok;
-  const int pmin = pos0 + min(wr0, it.nrows - 1) / a.group;
-  const int pmax = pos0 + min(wr0 + 31, it.nrows - 1) / a.group;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+  const uint32_t raw0 = lds0 + F::NTILE * STAGE;  // the ring of codes
+  const uint32_t ring0 = FP8 ? raw0 : lds0;
+  constexpr int RSTEP = FP8 ? F::RAW : STAGE;
+  if (tid < F::KW) s_odd[tid] = 0;
 
-  int page[2];
-  Codes<D, SHARED, TT> codes;
-  auto pages_for = [&](int st) {
-    constexpr int TW = TT / 4;
-#pragma unroll
-    for (int g = 0; g < (TW < 16 ? 1 : TW / 16); ++g)
-      page[g] = page_of(C, G, it, it.lo + st * TT + wave * TW + 16 * g);
-  };
-  auto check_pages = [&](int st) {  // a needed table entry that is no page
-    constexpr int TW = TT / 4;
-#pragma unroll
-    for (int g = 0; g < (TW < 16 ? 1 : TW / 16); ++g)
-    {
-      const int t = it.lo + st * TT + wave * TW + 16 * g;
-      if (t < it.hi && t + 15 >= it.clear && (page[g] < 0 || page[g] >= C.n_pages) && lane == 0)
-        atomicOr(C.status, DSV4G_CACHE_PAGE);
-    }
-  };
-  if (!FP8) {
-#pragma unroll
-    for (int i = 0; i < NBUF - 1; ++i)
-      if (it.s0 + i < it.s1) {
-        pages_for(it.s0 + i);
-        check_pages(it.s0 + i);
-        stage_bf16<D, SHARED, TT>(C, G, a, it, page, it.s0 + i, lds0 + i * STAGE, wave, lane);
-      }
+  Place w;
+  if (a.groups) {
+    attn_place<F::ROWS, TT>(C, a, w);
   } else {
-    pages_for(it.s0);
-    check_pages(it.s0);
-#pragma unroll
-    for (int i = 0; i < codes.H; ++i) {
-      codes.load(C, G, a, it, it.s0, i, wave, lane);
-      codes.store(lds, i, wave, lane);
-    }
+    int id = blockIdx.x;
+    w.kvh = id % C.kv_heads;
+    id /= C.kv_heads;
+    // the longest ranges first
+    w.pair = id % a.n_seqs * a.tiles + a.tiles - 1 - id / a.n_seqs;
+    w.stage = 0;
+    w.at = 0;
+    w.end = 1;
   }
-
-  // the query rows, once: columns 16 s + 8 h .. + 7 of row lane % 32; a
-  // negative scale is taken by their sign
-  Bf8 q[KS];
-  {
-    const size_t at = (size_t)(it.start + tok) * a.q_stride + (size_t)head * D + 8 * h;
-    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      U4 u;
-      if (a.f32) {
-        const float4 x = *(const float4 *)((const float *)a.q + at + 16 * s);
-        const float4 y = *(const float4 *)((const float *)a.q + at + 16 * s + 4);
-        u = U4{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w), pack_bf16(y.x, y.y),
-               pack_bf16(y.z, y.w)};
-      } else {
-        const uint4 x = *(const uint4 *)((const uint16_t *)a.q + at + 16 * s);
-        u = U4{x.x, x.y, x.z, x.w};
+  // One segment after the other: a run of stages of one item.
+  while (w.at < w.end) {
+    Item it;
+    if (!attn_item<F::ROWS, TT>(C, a, w.pair / a.tiles, w.pair % a.tiles, it)) {
+      if (!a.groups) return;
+      ++w.pair;  // no rows here
+      continue;
+    }
+    it.kvh = w.kvh;
+    const int s0 = w.stage;
+    const int s1 = a.groups ? (int)min((long)it.stages, s0 + w.end - w.at) : it.stages;
+    if (a.groups) {
+      if (s0 == 0 && tid == 0) {
+        a.first[1 + (long)w.pair * C.kv_heads + it.kvh] = w.at;
+        if (w.at == 0) a.first[0] = w.total;
       }
-      q[s] = __builtin_bit_cast(Bf8, u ^ sign);
-    }
-  }
-  const float c2 = fabsf(a.scale) * LOG2E;
-
-  F16v o[NP];
-#pragma unroll
-  for (int d = 0; d < NP; ++d) {
-    F16v y;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = 0.0f;
-    tile_in(o[d], y);
-  }
-  float m = -__builtin_inff(), l = 0.0f;  // l: this half's tokens
-  const uint32_t kat = lds0 + k_at<D>(lane) + 32 * kw * (2 * D);
-  const uint32_t vat = lds0 + v_at<D>(lane) + 32 * kw * (2 * D) + (SHARED ? 0 : F::KB);
-  // tokens that no row sees are not loaded; between these two are those that
-  // some row of the workgroup sees and another does not
-  const int shown = pos0 + it.r0 / a.group, hidden = it.hi - 1 - a.window;
-
-  for (int st = it.s0; st < it.s1; ++st) {
-    const int buf = (st - it.s0) % NBUF;
-    // stage st is in LDS for every wave, and every wave is done with the one before
-    if (!FP8) {
-      constexpr int PER = STAGE / 4096;  // direct loads per wave and stage
-      if (st + NBUF - 2 < it.s1) wait_loads<(NBUF - 2) * PER>();
-      else wait_loads<0>();
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const int next = st + (FP8 ? 1 : NBUF - 1);
-    const bool more = next < it.s1;
-    const uint32_t to = ((next - it.s0) % NBUF) * STAGE;
-    if (more) {
-      pages_for(next);
-      check_pages(next);
-      if (FP8) codes.load(C, G, a, it, next, 0, wave, lane);
-      else stage_bf16<D, SHARED, TT>(C, G, a, it, page, next, lds0 + to, wave, lane);
-    }
-    const int w0 = it.lo + st * TT;                 // the stage's tokens
-    const int t0 = w0 + 32 * kw;                    // this wave's 32
-    // 0 * NaN is NaN: where a token is hidden from some rows and not from
-    // others, its values are cleared if they are not all finite (a row that
-    // sees it is not finite then: by its score, or as below)
-    uint32_t odd = 0;
-    if (min(w0 + TT, it.hi) - 1 > shown || (a.window && max(w0, it.clear) <= hidden)) {
-      constexpr int PT = 256 / TT, NB = 2 * D / PT;  // threads per token, bytes of each
-      const int t = tid / PT;
-      const uint32_t at = lds0 + buf * STAGE + (SHARED ? 0 : F::KB) + t * (2 * D) +
-                          tid % PT * NB;
-      uint32_t big = 0;
-#pragma unroll
-      for (int j = 0; j < NB / 16; ++j) {
-        const U4 x = DSV4_LDS(U4, at + 16 * j);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          big |= ((x[k] & 0x7F80u) == 0x7F80u) | ((x[k] & 0x7F800000u) == 0x7F800000u);
+      w.at += s1 - s0;
+      w.stage = 0;
+      if (++w.kvh == C.kv_heads) {
+        w.kvh = 0;
+        ++w.pair;
       }
-      if (big) atomicOr(&s_odd[t / 32], 1u << (t % 32));
-      __syncthreads();
-      uint32_t any = 0;
-#pragma unroll
-      for (int k = 0; k < F::KW; ++k) any |= s_odd[k];
-      odd = __builtin_amdgcn_readfirstlane(any) ? 1u : 0u;
+    } else {
+      w.at = w.end;
     }
-    const bool none = !active || t0 > pmax || (a.window && t0 + 31 <= pmin - a.window);
-    Bf8 p0, p1;
-    if (!none) {
-      F16v z;
+    // this lane's row (the last one again where there are fewer)
+    const int wr0 = it.r0 + 32 * rw;
+    const bool active = wr0 < it.nrows;
+    const int r = min(wr0 + lane % 32, it.nrows - 1);
+    const int tok = r / a.group, head = it.kvh * a.group + r % a.group;
+    const int pos0 = it.len - it.count, pos = pos0 + tok;
+    const int pmin = pos0 + min(wr0, it.nrows - 1) / a.group;
+    const int pmax = pos0 + min(wr0 + 31, it.nrows - 1) / a.group;
+
+    Loader<D, SHARED, FP8, RW> load;
+    load.look(C, G, it, s0, wave);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) z[i] = 0.0f;
-      const uint32_t at = kat + buf * STAGE;
+    for (int i = 0; i < RING - 1; ++i)
+      if (s0 + i < s1) {
+        load.issue(C, G, a, it, s0 + i, ring0 + i * RSTEP, wave, lane);
+        load.look(C, G, it, s0 + i + 1, wave);
+      }
+
+    // the query rows, once: columns 16 s + 8 h .. + 7 of row lane % 32; a
+    // negative scale is taken by their sign
+    Bf8 q[KS];
+    {
+      const size_t at = (size_t)(it.start + tok) * a.q_stride + (size_t)head * D + 8 * h;
+      const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_k<D>(at, s), q[s], z, 0, 0, 0);
-        if (s % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // few reads ahead: registers
-      }
-      // token of z[i]: t0 + 8 (i / 4) + 4 h + i % 4
-      const bool mask = t0 + 31 > pmin || (a.window && t0 <= pmax - a.window);
-      if (mask) {
-        const int high = pos - t0 - 4 * h, low = a.window ? high - a.window : -64;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = 8 * (i / 4) + i % 4;
-          z[i] = at <= high && at > low ? z[i] : -__builtin_inff();
+        U4 u;
+        if (a.f32) {
+          const float4 x = *(const float4 *)((const float *)a.q + at + 16 * s);
+          const float4 y = *(const float4 *)((const float *)a.q + at + 16 * s + 4);
+          u = U4{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w), pack_bf16(y.x, y.y),
+                 pack_bf16(y.z, y.w)};
+        } else {
+          const uint4 x = *(const uint4 *)((const uint16_t *)a.q + at + 16 * s);
+          u = U4{x.x, x.y, x.z, x.w};
         }
-      }
-      float mx = z[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, z[i]);
-      mx = swap_max(mx);
-      const float mt = mx > -__builtin_inff() ? mx * c2 : -__builtin_inff();
-      if (__any(mt > m + AT_GROW)) {
-        const float M = fmaxf(m, mt);
-        const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
-        m = M;
-        l *= f;
-#pragma unroll
-        for (int d = 0; d < NP; ++d) {
-          F16v y = tile_out(o[d]);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] *= f;
-          tile_in(o[d], y);
-        }
-      }
-      const float mu = m > -__builtin_inff() ? m : 0.0f;
-      U4 b0, b1;
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        float x0 = __builtin_amdgcn_exp2f(fmaf(z[i], c2, -mu));
-        float x1 = __builtin_amdgcn_exp2f(fmaf(z[i + 1], c2, -mu));
-        if (mask) {  // a scale of 0 leaves -inf * 0
-          x0 = z[i] == -__builtin_inff() ? 0.0f : x0;
-          x1 = z[i + 1] == -__builtin_inff() ? 0.0f : x1;
-        }
-        l += x0 + x1;
-        if (i < 8) b0[i / 2] = pack_bf16(x0, x1);
-        else b1[i / 2 - 4] = pack_bf16(x0, x1);
-      }
-      p0 = __builtin_bit_cast(Bf8, b0);
-      p1 = __builtin_bit_cast(Bf8, b1);
-    }
-    if (FP8 && more) {
-      codes.store(lds + to, 0, wave, lane);
-      if (codes.H > 1) codes.load(C, G, a, it, next, 1, wave, lane);
-    }
-    if (odd) {
-      __syncthreads();  // every wave has its scores
-      const int t = tid % TT;
-      if (s_odd[t / 32] >> (t % 32) & 1) {
-        const uint32_t at = lds0 + buf * STAGE + (SHARED ? 0 : F::KB) + t * (2 * D);
-        for (int j = tid / TT; j < D / 8; j += 256 / TT)
-          DSV4_LDS(U4, at + 16 * j) = U4{0, 0, 0, 0};
-      }
-      for (uint32_t left = s_odd[kw]; left; left &= left - 1) {
-        const int t = t0 + __builtin_ctz(left);
-        if (t <= pos && (!a.window || t > pos - a.window)) l = __builtin_nanf("");
-      }
-      __syncthreads();
-      if (tid < F::KW) s_odd[tid] = 0;  // read again two barriers on at the earliest
-    }
-    if (!none) {
-      const uint32_t at = vat + buf * STAGE;
-#pragma unroll
-      for (int d = 0; d < NP; ++d) {
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_vt<D>(at, 0, d), p0, o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_vt<D>(at, 1, d), p1, o[d], 0, 0, 0);
+        q[s] = __builtin_bit_cast(Bf8, u ^ sign);
       }
     }
-    if (FP8 && more && codes.H > 1) codes.store(lds + to, 1, wave, lane);
-  }
-  l = swap_sum(l);
+    const float c2 = fabsf(a.scale) * LOG2E;
 
-  // the waves that shared the rows: into the first one, through LDS
-  if constexpr (F::KW > 1) {
-    constexpr int PART = F::PART;
-    for (int k = 1; k < F::KW; ++k) {
-      __syncthreads();
-      float4 *w = (float4 *)(lds + rw * PART);
-      float2 *ws = (float2 *)(lds + rw * PART + 32 * D * 4);
-      if (kw == k) {
+    F16v o[NP];
+#pragma unroll
+    for (int d = 0; d < NP; ++d) {
+      F16v y;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = 0.0f;
+      tile_in(o[d], y);
+    }
+    float m = -__builtin_inff(), l = 0.0f;  // l: this half's tokens
+    const uint32_t kat = lds0 + k_at<D>(lane) + 32 * kw * (2 * D);
+    const uint32_t vat = lds0 + v_at<D>(lane) + 32 * kw * (2 * D) + (SHARED ? 0 : F::KB);
+    // tokens that no row sees are not loaded; between these two are those that
+    // some row of the workgroup sees and another does not
+    const int shown = pos0 + it.r0 / a.group, hidden = it.hi - 1 - a.window;
+
+    if (F::TWICE) {  // the first stage's rows
+      wait_loads<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      convert<D, SHARED, TT>(raw0, lds0, tid);
+    }
+    for (int st = s0; st < s1; ++st) {
+      const int i = st - s0;
+      // what is read of the ring below (stage st; st + 1 where it is converted
+      // ahead) is in LDS for every wave, and every wave is done with the stage
+      // before st
+      constexpr int AHEAD = F::TWICE ? 1 : 0;
+      if (st + RING - 2 < s1) wait_loads<(RING - 2 - AHEAD) * F::PER>();
+      else wait_loads<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (FP8 && !F::TWICE) {
+        convert<D, SHARED, TT>(raw0 + i % RING * RSTEP, lds0, tid);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      const int next = st + RING - 1;
+      if (next < s1) {
+        load.issue(C, G, a, it, next, ring0 + (i + RING - 1) % RING * RSTEP, wave, lane);
+        load.look(C, G, it, next + 1, wave);
+      }
+      const uint32_t here = i % F::NTILE * STAGE;  // the stage's rows
+      const int w0 = it.lo + st * TT;                 // the stage's tokens
+      const int t0 = w0 + 32 * kw;                    // this wave's 32
+      // 0 * NaN is NaN: where a token is hidden from some rows and not from
+      // others, its values are cleared if they are not all finite (a row that
+      // sees it is not finite then: by its score, or as below)
+      uint32_t odd = 0;
+      if (min(w0 + TT, it.hi) - 1 > shown || (a.window && max(w0, it.clear) <= hidden)) {
+        constexpr int PT = 256 / TT, NB = 2 * D / PT;  // threads per token, bytes of each
+        const int t = tid / PT;
+        const uint32_t at = lds0 + here + (SHARED ? 0 : F::KB) + t * (2 * D) +
+                            tid % PT * NB;
+        uint32_t big = 0;
+#pragma unroll
+        for (int j = 0; j < NB / 16; ++j) {
+          const U4 x = DSV4_LDS(U4, at + 16 * j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            big |= ((x[k] & 0x7F80u) == 0x7F80u) | ((x[k] & 0x7F800000u) == 0x7F800000u);
+        }
+        if (big) atomicOr(&s_odd[t / 32], 1u << (t % 32));
+        __syncthreads();
+        uint32_t any = 0;
+#pragma unroll
+        for (int k = 0; k < F::KW; ++k) any |= s_odd[k];
+        odd = __builtin_amdgcn_readfirstlane(any) ? 1u : 0u;
+      }
+      const bool none = !active || t0 > pmax || (a.window && t0 + 31 <= pmin - a.window);
+      Bf8 p0, p1;
+      if (!none) {
+        F16v z;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+        const uint32_t at = kat + here;
+        // reads a few steps ahead of the products that take them
+        constexpr int R = AT_AHEAD;
+        __builtin_amdgcn_sched_barrier(0);
+        Bf8 k[R];
+#pragma unroll
+        for (int s = 0; s < R && s < KS; ++s) k[s] = read_k<D>(at, s);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[s % R], q[s], z, 0, 0, 0);
+          if (s + R < KS) k[s % R] = read_k<D>(at, s + R);
+        }
+        sched_steps<KS, R, 1, 1>();
+        __builtin_amdgcn_sched_barrier(0);
+        // token of z[i]: t0 + 8 (i / 4) + 4 h + i % 4
+        const bool mask = t0 + 31 > pmin || (a.window && t0 <= pmax - a.window);
+        if (mask) {
+          const int high = pos - t0 - 4 * h, low = a.window ? high - a.window : -64;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = 8 * (i / 4) + i % 4;
+            z[i] = at <= high && at > low ? z[i] : -__builtin_inff();
+          }
+        }
+        float mx = z[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, z[i]);
+        mx = swap_max(mx);
+        const float mt = mx > -__builtin_inff() ? mx * c2 : -__builtin_inff();
+        if (__any(mt > m + AT_GROW)) {
+          const float M = fmaxf(m, mt);
+          const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
+          m = M;
+          l *= f;
+#pragma unroll
+          for (int d = 0; d < NP; ++d) {
+            F16v y = tile_out(o[d]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] *= f;
+            tile_in(o[d], y);
+          }
+        }
+        const float mu = m > -__builtin_inff() ? m : 0.0f;
+        U4 b0, b1;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float x0 = __builtin_amdgcn_exp2f(fmaf(z[i], c2, -mu));
+          float x1 = __builtin_amdgcn_exp2f(fmaf(z[i + 1], c2, -mu));
+          if (mask) {  // a scale of 0 leaves -inf * 0
+            x0 = z[i] == -__builtin_inff() ? 0.0f : x0;
+            x1 = z[i + 1] == -__builtin_inff() ? 0.0f : x1;
+          }
+          l += x0 + x1;
+          if (i < 8) b0[i / 2] = pack_bf16(x0, x1);
+          else b1[i / 2 - 4] = pack_bf16(x0, x1);
+        }
+        p0 = __builtin_bit_cast(Bf8, b0);
+        p1 = __builtin_bit_cast(Bf8, b1);
+      }
+      if (F::TWICE && st + 1 < s1)
+        convert<D, SHARED, TT>(raw0 + (i + 1) % RING * RSTEP, lds0 + (i + 1) % 2 * STAGE, tid);
+      if (odd) {
+        __syncthreads();  // every wave has its scores
+        const int t = tid % TT;
+        if (s_odd[t / 32] >> (t % 32) & 1) {
+          const uint32_t at = lds0 + here + (SHARED ? 0 : F::KB) + t * (2 * D);
+          for (int j = tid / TT; j < D / 8; j += 256 / TT)
+            DSV4_LDS(U4, at + 16 * j) = U4{0, 0, 0, 0};
+        }
+        for (uint32_t left = s_odd[kw]; left; left &= left - 1) {
+          const int t = t0 + __builtin_ctz(left);
+          if (t <= pos && (!a.window || t > pos - a.window)) l = __builtin_nanf("");
+        }
+        __syncthreads();
+        if (tid < F::KW) s_odd[tid] = 0;  // read again two barriers on at the earliest
+      }
+      if (!none) {
+        const uint32_t at = vat + here;
+        constexpr int R = AT_AHEAD / 2;
+        __builtin_amdgcn_sched_barrier(0);
+        Bf8 v[2 * R];
+#pragma unroll
+        for (int s = 0; s < 2 * R && s < 2 * NP; ++s) v[s] = read_vt<D>(at, s % 2, s / 2);
+#pragma unroll
+        for (int s = 0; s < 2 * NP; ++s) {
+          o[s / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[s % (2 * R)], s % 2 ? p1 : p0,
+                                                             o[s / 2], 0, 0, 0);
+          if (s + 2 * R < 2 * NP)
+            v[s % (2 * R)] = read_vt<D>(at, s % 2, (s + 2 * R) / 2);
+        }
+        sched_steps<2 * NP, 2 * R, 1, 2>();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    l = swap_sum(l);
+
+    // the waves that shared the rows: into the first one, through LDS
+    if constexpr (F::KW > 1) {
+      constexpr int PART = F::PART;
+      for (int k = 1; k < F::KW; ++k) {
+        __syncthreads();
+        float4 *x = (float4 *)(lds + rw * PART);
+        float2 *xs = (float2 *)(lds + rw * PART + 32 * D * 4);
+        if (kw == k) {
+#pragma unroll
+          for (int d = 0; d < NP; ++d) {
+            const F16v y = tile_out(o[d]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              x[(4 * d + g) * 64 + lane] =
+                  make_float4(y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          xs[lane] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (kw == 0) {
+          const float2 s = xs[lane];
+          const float M = fmaxf(m, s.x);
+          const bool any = M > -__builtin_inff();
+          const float f0 = any ? exp2f(m - M) : 1.0f, f1 = any ? exp2f(s.x - M) : 0.0f;
+          l = l * f0 + s.y * f1;
+          m = M;
+#pragma unroll
+          for (int d = 0; d < NP; ++d) {
+            F16v y = tile_out(o[d]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float4 p = x[(4 * d + g) * 64 + lane];
+              y[4 * g] = y[4 * g] * f0 + p.x * f1;
+              y[4 * g + 1] = y[4 * g + 1] * f0 + p.y * f1;
+              y[4 * g + 2] = y[4 * g + 2] * f0 + p.z * f1;
+              y[4 * g + 3] = y[4 * g + 3] * f0 + p.w * f1;
+            }
+            tile_in(o[d], y);
+          }
+        }
+      }
+    }
+    if (kw == 0 && active && wr0 + lane % 32 < it.nrows) {
+      if (s0 > 0 || s1 < it.stages) {
+        const size_t slot = 2 * (size_t)blockIdx.x + (s0 == 0);  // the run's last item, or its first
+        float4 *to = (float4 *)(a.part + (slot * F::ROWS + 32 * rw) * D);
 #pragma unroll
         for (int d = 0; d < NP; ++d) {
           const F16v y = tile_out(o[d]);
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            w[(4 * d + g) * 64 + lane] =
+            to[(4 * d + g) * 64 + lane] =
                 make_float4(y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]);
           __builtin_amdgcn_sched_barrier(0);
         }
-        ws[lane] = make_float2(m, l);
-      }
-      __syncthreads();
-      if (kw == 0) {
-        const float2 s = ws[lane];
-        const float M = fmaxf(m, s.x);
-        const bool any = M > -__builtin_inff();
-        const float f0 = any ? exp2f(m - M) : 1.0f, f1 = any ? exp2f(s.x - M) : 0.0f;
-        l = l * f0 + s.y * f1;
-        m = M;
+        if (h == 0) a.stat[slot * F::ROWS + 32 * rw + lane] = make_float2(m, l);
+      } else {
+        float lse;
+        const float f = finish_row(a, head, m, l, &lse);
+        const size_t row = (size_t)(it.start + tok);
 #pragma unroll
         for (int d = 0; d < NP; ++d) {
-          F16v y = tile_out(o[d]);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float4 x = w[(4 * d + g) * 64 + lane];
-            y[4 * g] = y[4 * g] * f0 + x.x * f1;
-            y[4 * g + 1] = y[4 * g + 1] * f0 + x.y * f1;
-            y[4 * g + 2] = y[4 * g + 2] * f0 + x.z * f1;
-            y[4 * g + 3] = y[4 * g + 3] * f0 + x.w * f1;
-          }
-          tile_in(o[d], y);
+          store_tile<D>(a, row * a.out_stride + (size_t)head * D, d, h, tile_out(o[d]), f);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        if (a.lse && h == 0) a.lse[row * a.heads + head] = lse;
       }
     }
-    if (kw) return;
+    if (!a.groups) return;
+    __syncthreads();  // the stages' LDS is free again
   }
-  if (!active || wr0 + lane % 32 >= it.nrows) return;
-  if (it.parts > 1) {
-    float4 *w = (float4 *)(a.part + ((size_t)blockIdx.x * F::ROWS + 32 * rw) * D);
-#pragma unroll
-    for (int d = 0; d < NP; ++d) {
-      const F16v y = tile_out(o[d]);
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        w[(4 * d + g) * 64 + lane] =
-            make_float4(y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (h == 0) a.stat[(size_t)blockIdx.x * F::ROWS + 32 * rw + lane] = make_float2(m, l);
-    return;
-  }
-  float lse;
-  const float f = finish_row(a, head, m, l, &lse);
-  const size_t row = (size_t)(it.start + tok);
-#pragma unroll
-  for (int d = 0; d < NP; ++d) {
-    store_tile<D>(a, row * a.out_stride + (size_t)head * D, d, h, tile_out(o[d]), f);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  if (a.lse && h == 0) a.lse[row * a.heads + head] = lse;
 }
 
-// Joins the parts of every split item: one wave per output tile of a row wave.
+// Joins the parts of every item that several workgroups shared: one wave per
+// output tile of a row wave.
 template <int D, int RW>
 __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   constexpr int TT = 32 * (4 / RW), ROWS = 32 * RW, NP = D / 32;
@@ -662,36 +853,41 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   const int d = id % NP;
   id /= NP;
   const int rw = id % RW;
-  id /= RW;
-  if (id >= a.items) return;
+  id /= RW;  // (sequence, tile), kv head
+  const int kvh = id % C.kv_heads, pair = id / C.kv_heads;
+  if (pair >= a.n_seqs * a.tiles) return;
   Item it;
-  if (!attn_item<ROWS, TT>(C, a, id * a.nsplit, it) || it.parts == 1) return;
+  if (!attn_item<ROWS, TT>(C, a, pair / a.tiles, pair % a.tiles, it)) return;
+  const long total = a.first[0], at = a.first[1 + id];
+  const int groups = shared_groups(a, total);
+  const int w0 = share_of(total, groups, at), w1 = share_of(total, groups, at + it.stages - 1);
   const int r = it.r0 + 32 * rw + lane % 32;
-  if (r >= it.nrows) return;
-  const size_t first = (size_t)id * a.nsplit;
-  const float2 *stat = a.stat + first * ROWS + 32 * rw + lane % 32;
+  if (w0 == w1 || r >= it.nrows) return;
+  // the first workgroup's part is its run's last, the others' their first
+  auto slot = [&](int w) { return (2 * (size_t)w + (w == w0)) * ROWS + 32 * rw; };
   float m = -__builtin_inff(), l = 0.0f;
-  for (int p = 0; p < it.parts; ++p) m = fmaxf(m, stat[(size_t)p * ROWS].x);
+#pragma unroll 4
+  for (int w = w0; w <= w1; ++w) m = fmaxf(m, a.stat[slot(w) + lane % 32].x);
   const float mu = m > -__builtin_inff() ? m : 0.0f;
   F16v o;
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = 0.0f;
 #pragma unroll 4
-  for (int p = 0; p < it.parts; ++p) {
-    const float2 s = stat[(size_t)p * ROWS];
-    const float f = exp2f(s.x - mu);
+  for (int w = w0; w <= w1; ++w) {
+    const float2 s = a.stat[slot(w) + lane % 32];
+    const float f = __builtin_amdgcn_exp2f(s.x - mu);
     l += s.y * f;
-    const float4 *w = (const float4 *)(a.part + ((first + p) * ROWS + 32 * rw) * D);
+    const float4 *from = (const float4 *)(a.part + slot(w) * D);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 x = w[(4 * d + g) * 64 + lane];
+      const float4 x = from[(4 * d + g) * 64 + lane];
       o[4 * g] += x.x * f;
       o[4 * g + 1] += x.y * f;
       o[4 * g + 2] += x.z * f;
       o[4 * g + 3] += x.w * f;
     }
   }
-  const int tok = r / a.group, head = it.kvh * a.group + r % a.group;
+  const int tok = r / a.group, head = kvh * a.group + r % a.group;
   float lse;
   const float f = finish_row(a, head, m, l, &lse);
   const size_t row = (size_t)(it.start + tok);
@@ -701,16 +897,19 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
 
 // ------------------------------------------------------------- launch plan
 struct AttnPlan {
-  int rw, tiles, nsplit;
+  int rw, tiles, groups;
   long items;
   size_t bytes;
 };
-static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_tokens, int max_q,
-                          int max_kv, int window) {
+template <int D, bool SHARED>
+static int attn_places(int rw, bool fp8) {  // workgroups that the chip holds
+  return 256 * (rw == 1   ? (fp8 ? Cfg<D, SHARED, true, 1>::WGS : Cfg<D, SHARED, false, 1>::WGS)
+                : rw == 2 ? (fp8 ? Cfg<D, SHARED, true, 2>::WGS : Cfg<D, SHARED, false, 2>::WGS)
+                          : (fp8 ? Cfg<D, SHARED, true, 4>::WGS : Cfg<D, SHARED, false, 4>::WGS));
+}
+static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_tokens, int max_q) {
   AttnPlan p;
-  const long room = (long)C->max_pages * C->page_size;
   max_q = max_q > n_tokens ? n_tokens : max_q;
-  max_kv = max_kv > room ? (int)room : max_kv;
   const long rows = (long)max_q * (heads / C->kv_heads);
   const int D = C->k_dim;
   // the smallest tile that holds a sequence's rows
@@ -719,17 +918,16 @@ static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_toke
   p.rw = p.rw < least ? least : p.rw;
   p.tiles = (int)((rows + 32 * p.rw - 1) / (32 * p.rw));
   p.items = (long)p.tiles * n_seqs * C->kv_heads;
-  const int tt = 32 * (4 / p.rw);
-  long range = max_kv;
-  if (window && (long)window + 32L * p.rw < range) range = window + 32L * p.rw;
-  const long slots = 256L * (D <= 128 ? 2 : 1);
-  long want = slots / p.items;
-  const long most = (range + 2 * tt - 1) / (2 * tt);
-  want = want > most ? most : want;
-  want = want > AT_MAX_SPLIT ? AT_MAX_SPLIT : want;
-  p.nsplit = want < 1 ? 1 : (int)want;
-  const size_t cells = (size_t)p.items * p.nsplit * 32 * p.rw;
-  p.bytes = p.nsplit > 1 ? cells * (D * sizeof(float) + sizeof(float2)) : 0;
+  const bool fp8 = C->dtype == DSV4G_DT_F8_E4M3;
+  const int places = D == 64    ? attn_places<64, false>(p.rw, fp8)
+                     : D == 128 ? attn_places<128, false>(p.rw, fp8)
+                                : 256;
+  // two items per place and more: each whole; fewer: their stages dealt out
+  p.groups = p.items < 2 * places ? places : 0;
+  p.bytes = 0;
+  if (p.groups)
+    p.bytes = (size_t)p.groups * 2 * 32 * p.rw * (D * sizeof(float) + sizeof(float2)) +
+              (1 + (size_t)p.items) * sizeof(long);
   return p;
 }
 
@@ -737,9 +935,9 @@ template <int D, bool SHARED, bool FP8, int RW>
 static void attn_launch(const DSV4GCache &C, const CacheGeom &G, const AttnArgs &a, long items,
                         hipStream_t st) {
   if constexpr (Cfg<D, SHARED, FP8, RW>::OK) {
-    hipLaunchKernelGGL((k_attn<D, SHARED, FP8, RW>), dim3((unsigned)(items * a.nsplit)), dim3(256),
-                       0, st, C, G, a);
-    if (a.nsplit > 1)
+    hipLaunchKernelGGL((k_attn<D, SHARED, FP8, RW>), dim3((unsigned)(a.groups ? a.groups : items)),
+                       dim3(256), 0, st, C, G, a);
+    if (a.groups)
       hipLaunchKernelGGL((k_attn_join<D, RW>), dim3((unsigned)((items * RW * (D / 32) + 3) / 4)),
                          dim3(256), 0, st, C, a);
   }
@@ -767,7 +965,7 @@ size_t dsv4g_attention_workspace_bytes(const DSV4GCache *C, int heads, int n_seq
   if (!C || !cache_geom(C, &G) || heads <= 0 || heads % C->kv_heads || n_seqs <= 0 ||
       n_tokens <= 0 || max_q <= 0 || max_kv <= 0)
     return 0;
-  return attn_plan(C, heads, n_seqs, n_tokens, max_q, max_kv, 0).bytes;
+  return attn_plan(C, heads, n_seqs, n_tokens, max_q).bytes;
 }
 
 int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, size_t q_stride,
@@ -788,8 +986,8 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
       q_stride % unit || out_stride % unit || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))
     return dsv4g_fail(DSV4G_EINVAL, "attention: rows of q and out must be 16-byte aligned and at "
                       "least heads * dim apart");
-  const AttnPlan p = attn_plan(C, heads, n_seqs, n_tokens, max_q, max_kv, window);
-  if (p.items * p.nsplit > 0x7FFFFFFFL || (long)max_q * (heads / C->kv_heads) > 0x7FFFFF00L)
+  const AttnPlan p = attn_plan(C, heads, n_seqs, n_tokens, max_q);
+  if (p.items > 0x7FFFFFFFL || (long)max_q * (heads / C->kv_heads) > 0x7FFFFF00L)
     return dsv4g_fail(DSV4G_EINVAL, "attention: too many rows for one call");
   if (p.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.bytes))
     return dsv4g_fail(DSV4G_EINVAL, "attention: 256-byte aligned workspace of %zu bytes needed "
@@ -799,9 +997,13 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
   a.seqs = seqs, a.starts = starts, a.sink = sink, a.layer = layer, a.heads = heads;
   a.group = heads / C->kv_heads, a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.max_q = max_q;
   a.max_kv = max_kv, a.window = window, a.f32 = act_dtype == DSV4G_DT_F32;
-  a.tiles = p.tiles, a.nsplit = p.nsplit, a.items = (int)p.items, a.scale = scale;
-  a.part = (float *)workspace;
-  if (p.nsplit > 1) a.stat = (float2 *)(a.part + (size_t)p.items * p.nsplit * 32 * p.rw * C->k_dim);
+  a.tiles = p.tiles, a.groups = p.groups, a.scale = scale;
+  if (p.groups) {
+    const size_t cells = (size_t)p.groups * 2 * 32 * p.rw;
+    a.part = (float *)workspace;
+    a.stat = (float2 *)(a.part + cells * C->k_dim);
+    a.first = (long *)(a.stat + cells);
+  }
   const hipStream_t st = (hipStream_t)stream;
   const bool shared = C->v_dim == 0;
   switch (C->k_dim) {
