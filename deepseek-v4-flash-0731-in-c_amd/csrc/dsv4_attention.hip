@@ -23,11 +23,23 @@
 // Rows of 16-byte chunks are stored with the chunk index XORed by a function
 // of the row (chunk_swizzle): both kinds of read then touch every bank once
 // per 16 lanes.
+#include <utility>
+
 #include "dsv4_cache.h"
 #include "dsv4_device.h"
 #include "dsv4_gpu_internal.h"
 
 namespace dsv4 {
+
+// f(0), .., f(N - 1), each with its number as a constant.
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F &f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F &&f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
 
 typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
 typedef float F16v __attribute__((ext_vector_type(16)));
@@ -133,6 +145,19 @@ __device__ __forceinline__ bool attn_item(const DSV4GCache &C, const AttnArgs &a
   return true;
 }
 
+// Values that are the same in every lane, in scalar registers: the compiler
+// would else keep what came through LDS or a vector load, and all that is
+// computed from it, in vector registers.
+__device__ __forceinline__ int one(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long one(long x) {
+  return (long)(((uint64_t)(uint32_t)one((int)(x >> 32)) << 32) | (uint32_t)one((int)x));
+}
+__device__ __forceinline__ void one(Item &it) {
+  int *f = &it.b;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(Item) / sizeof(int)); ++i) f[i] = one(f[i]);
+}
+
 // Shared work (fewer items than the chip has places for): the stages of all
 // items in a row, items ordered by (sequence, tile), then kv head, are dealt
 // out in equal runs, so that long and short sequences fill every workgroup
@@ -179,7 +204,7 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
     total += s_sum[w];
   }
   before *= C.kv_heads;
-  p.total = total * C.kv_heads;
+  p.total = one(total * C.kv_heads);
   const int groups = shared_groups(a, p.total);
   p.at = p.end = 0;
   if ((int)blockIdx.x >= groups) return;
@@ -210,126 +235,128 @@ __device__ __forceinline__ void fresh(int &x) { asm volatile("" : "+v"(x)); }
 // Direct loads to LDS, 16 or 4 bytes per lane (lane l's at `to` + its size *
 // l). In inline asm: they have no output register, and the compiler would make
 // every later LDS read wait for all of them; wait_loads() and the barrier
-// order them instead.
+// order them instead (what they write is read behind the next ones only).
 __device__ __forceinline__ void lds_load16(uint32_t to, uint32_t at, I4 rsrc) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               ::"s"(to), "v"(at), "s"(rsrc)
-               : "memory");
+               ::"s"(to), "v"(at), "s"(rsrc));
 }
 __device__ __forceinline__ void lds_load4(uint32_t to, uint32_t at, I4 rsrc) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               ::"s"(to), "v"(at), "s"(rsrc)
-               : "memory");
+               ::"s"(to), "v"(at), "s"(rsrc));
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ I4 page_rsrc(const DSV4GCache &C, const CacheGeom &G, int layer,
-                                        int page) {
-  const bool ok = page >= 0 && page < C.n_pages;
-  const uint64_t p = (uint64_t)(uintptr_t)C.pages +
-                     ((uint64_t)layer * C.n_pages + (ok ? page : 0)) * G.page_bytes;
-  // no bytes behind a page that is none: its loads give zeros
-  return I4{(int)(uint32_t)p, (int)(uint32_t)(p >> 32), ok ? (int)G.page_bytes : 0, 0x00020000};
-}
-
-// Brings stages of an item to LDS. Each wave brings a quarter of the tokens in
-// one or two groups of at most 16 (one page each); the pages of a stage are
-// looked up while the one before it is issued.
+// Brings stages of an item to LDS, PER loads per wave: begin() looks at the
+// pages, load(k) issues one. A stage behind the last (`st` < 0) is loads that
+// bring zeros, so that the loop has no branch and its waits count alike.
+// The pages of a stage are looked up one stage ahead.
 constexpr uint32_t AT_OUT = 0x7FFFFFFFu;  // an offset behind any page: zeros
 template <int D, bool SHARED, bool FP8, int RW>
 struct Loader {
   typedef Cfg<D, SHARED, FP8, RW> F;
-  // tokens of a wave's group, groups: E4M3 with narrow heads needs 16 tokens
-  // for one load, which the waves then bring twice
-  static constexpr int TT = F::TT, TW = TT / 4;
-  static constexpr int TG = FP8 ? (1024 / D > TW ? 1024 / D : at_min(16, TW)) : at_min(16, TW);
-  static constexpr int NG = at_max(1, TW / TG);
-  int page[NG];
-  __device__ __forceinline__ int first(int wave, int g) const {
-    return (wave * NG + g) * TG % TT;  // the stage's token where group g begins
+  // Rows: a wave brings a quarter of the tokens, NG groups of TG (one page
+  // each), TB per load. E4M3 with narrow heads: 16 tokens are one load, which
+  // two waves then bring alike.
+  static constexpr int TT = F::TT, TW = TT / 4, M = F::M;
+  static constexpr int TB = FP8 ? 1024 / D : 512 / D;
+  static constexpr int TG = at_max(at_min(16, TW), TB), NG = at_max(1, TW / TG);
+  static constexpr int ROWS_PER = NG * (TG / TB);
+  // Scale codes: 16 tokens per load, 4 bytes per lane
+  static constexpr int NS = FP8 ? at_max(1, TT / 64) : 0;
+  static_assert(F::PER == M * (ROWS_PER + NS), "loads of a stage");
+  int page[NG], spage[at_max(1, NS)];  // of the next stage
+  I4 rsrc[NG], srsrc[at_max(1, NS)];   // of this one
+  int t0, w0;                          // its first token, the wave's of it
+  uint32_t lds;
+
+  __device__ __forceinline__ int row_group(int wave, int g) const {
+    return (wave * NG + g) * TG % TT;
   }
-  __device__ __forceinline__ bool needed(const Item &it, int t) const {
-    return t < it.hi && t + TG > it.clear;
+  __device__ __forceinline__ int scale_group(int wave, int k) const {
+    return (wave * NS + k) * 16 % TT;
+  }
+  __device__ __forceinline__ int page_of(const DSV4GCache &C, const CacheGeom &G, const Item &it,
+                                         int t, int n) const {
+    if (t >= it.hi || t + n <= it.clear) return -2;  // nothing is needed of it
+    const int *cell = C.table + (size_t)it.seq * C.max_pages + (t >> G.shift);
+    // written by earlier kernels only: a scalar load
+    const int page = *(const __attribute__((address_space(4))) int *)cell;
+    return page < 0 || page >= C.n_pages ? -1 : page;
   }
   __device__ __forceinline__ void look(const DSV4GCache &C, const CacheGeom &G, const Item &it,
                                        int st, int wave) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int t = it.lo + st * TT + first(wave, g);
-      page[g] = -1;
-      if (needed(it, t)) {
-        const int *cell = C.table + (size_t)it.seq * C.max_pages + (t >> G.shift);
-        // written by earlier kernels only
-        page[g] = *(const __attribute__((address_space(4))) int *)cell;
-      }
-    }
+    for (int g = 0; g < NG; ++g)
+      page[g] = page_of(C, G, it, it.lo + st * TT + row_group(wave, g), TG);
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+      spage[k] = page_of(C, G, it, it.lo + st * TT + scale_group(wave, k), 16);
   }
-  __device__ __forceinline__ void issue(const DSV4GCache &C, const CacheGeom &G, const AttnArgs &a,
-                                        const Item &it, int st, uint32_t lds, int wave, int lane) {
+  __device__ __forceinline__ I4 page_rsrc(const DSV4GCache &C, const CacheGeom &G, int layer,
+                                          int page, bool live) const {
+    const uint64_t p = (uint64_t)(uintptr_t)C.pages +
+                       ((uint64_t)layer * C.n_pages + (page < 0 ? 0 : page)) * G.page_bytes;
+    return I4{(int)(uint32_t)p, (int)(uint32_t)(p >> 32),
+              live && page >= 0 ? (int)G.page_bytes : 0, 0x00020000};
+  }
+  __device__ __forceinline__ void begin(const DSV4GCache &C, const CacheGeom &G, const AttnArgs &a,
+                                        const Item &it, int st, bool live, uint32_t to,
+                                        int wave) {
+    lds = to;
+    t0 = it.lo + st * TT;
+    bool bad = false;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      bad |= page[g] == -1;
+      rsrc[g] = page_rsrc(C, G, a.layer, page[g], live);
+    }
+#pragma unroll
+    for (int k = 0; k < NS; ++k) srsrc[k] = page_rsrc(C, G, a.layer, spage[k], live);
+    if (live && bad && threadIdx.x % 64 == 0) atomicOr(C.status, DSV4G_CACHE_PAGE);
+    look(C, G, it, st + 1, wave);
+  }
+  template <int K>
+  __device__ __forceinline__ void load(const DSV4GCache &C, const CacheGeom &G, const Item &it,
+                                       int wave, int lane) const {
     fresh(lane);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int tl0 = first(wave, g);
-      const int t0 = it.lo + st * TT + tl0;  // token of the sequence
-      if (needed(it, t0) && (page[g] < 0 || page[g] >= C.n_pages) && lane == 0)
-        atomicOr(C.status, DSV4G_CACHE_PAGE);
-      const I4 rsrc = page_rsrc(C, G, a.layer, page[g]);
-      const int slot = it.kvh * C.page_size + (t0 & (C.page_size - 1));
-      auto in = [&](int off) { return t0 + off < it.hi && t0 + off >= it.clear; };
-      if (!FP8) {
-        constexpr int CH = D / 8, TB = 64 / CH;  // chunks of a row, tokens per load
-#pragma unroll
-        for (int j = 0; j < TG / TB; ++j) {
-          const int off = j * TB + lane / CH;
-          const uint32_t v = (uint32_t)(slot + off) * (2 * D) +
-                             16u * ((lane % CH) ^ chunk_swizzle<D>(tl0 + off));
-          const uint32_t to = lds + (tl0 + j * TB) * (2 * D);
-          lds_load16(to, in(off) ? v : AT_OUT, rsrc);
-          if (!SHARED) lds_load16(to + F::KB, in(off) ? v + G.v_off : AT_OUT, rsrc);
-        }
+    constexpr int m = K % M, i = K / M;
+    const int head = it.kvh * C.page_size, mask = C.page_size - 1;
+    if constexpr (i < ROWS_PER) {
+      constexpr int g = i / (TG / TB), j = i % (TG / TB);
+      const int tl0 = row_group(wave, g), off = j * TB + lane * TB / 64;
+      const int slot = head + ((t0 + tl0) & mask) + off, tok = t0 + tl0 + off;
+      const bool in = tok < it.hi && tok >= it.clear;
+      uint32_t v, to;
+      if (FP8) {
+        v = (uint32_t)slot * D + lane * 16 % D;
+        to = lds + (tl0 + j * TB) * D + m * (F::CODES + F::SCALES);
       } else {
-        constexpr int TB = 1024 / D;  // tokens per load
-#pragma unroll
-        for (int j = 0; j < TG / TB; ++j) {
-          const int off = j * TB + lane * 16 / D;
-          const uint32_t v = (uint32_t)(slot + off) * D + lane * 16 % D;
-          const uint32_t to = lds + (tl0 + j * TB) * D;
-          lds_load16(to, in(off) ? v : AT_OUT, rsrc);
-          if (!SHARED) lds_load16(to + F::CODES + F::SCALES, in(off) ? v + G.v_off : AT_OUT, rsrc);
-        }
+        constexpr int CH = D / 8;
+        v = (uint32_t)slot * (2 * D) + 16u * ((lane % CH) ^ chunk_swizzle<D>(tl0 + off));
+        to = lds + (tl0 + j * TB) * (2 * D) + m * F::KB;
       }
+      lds_load16(to, in ? v + (m ? G.v_off : 0) : AT_OUT, rsrc[g]);
+    } else {
+      constexpr int S = D / 64, LANES = 4 * S;  // codes of a token, lanes of a load
+      const int tl0 = scale_group(wave, i - ROWS_PER);
+      const int slot = head + ((t0 + tl0) & mask), tok = t0 + tl0 + 4 * lane / S;
+      constexpr int SPAN = S < 4 ? 4 / S : 1;   // tokens of a lane's 4 bytes
+      const bool in = tok < it.hi && tok + SPAN > it.clear;
+      const uint32_t v = (uint32_t)slot * S + 4 * lane + (m ? G.vs_off : G.ks_off);
+      if (lane < LANES)
+        lds_load4(lds + F::CODES + tl0 * S + m * (F::CODES + F::SCALES), in ? v : AT_OUT,
+                  srsrc[i - ROWS_PER]);
     }
-    if (FP8) scales(C, G, a, it, st, lds, wave, lane);
   }
-  // Scale codes, 16 tokens per load (4 bytes per lane): their group g16 has a
-  // page of its own lookup where the wave's codes lie in another page.
-  __device__ __forceinline__ void scales(const DSV4GCache &C, const CacheGeom &G,
-                                         const AttnArgs &a, const Item &it, int st, uint32_t lds,
-                                         int wave, int lane) {
-    constexpr int N = at_max(1, TT / 64), L = 4 * (D / 64);  // loads per wave, lanes of one
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int tl0 = (wave * N + k) * 16 % TT;
-      const int t0 = it.lo + st * TT + tl0;
-      int pg = -1;
-      if (t0 < it.hi && t0 + 16 > it.clear) {
-        const int *cell = C.table + (size_t)it.seq * C.max_pages + (t0 >> G.shift);
-        pg = *(const __attribute__((address_space(4))) int *)cell;
-      }
-      const I4 rsrc = page_rsrc(C, G, a.layer, pg);
-      const int slot = it.kvh * C.page_size + (t0 & (C.page_size - 1));
-      const int off = 4 * lane / (D / 64);  // token of this lane's first code
-      const bool some = t0 + off < it.hi && t0 + off + (D < 256 ? 256 / D : 1) > it.clear;
-      const uint32_t v = some ? (uint32_t)slot * (D / 64) + 4 * lane : AT_OUT;
-      const uint32_t to = lds + F::CODES + tl0 * (D / 64);
-      if (lane < L) {
-        lds_load4(to, some ? v + G.ks_off : AT_OUT, rsrc);
-        if (!SHARED) lds_load4(to + F::CODES + F::SCALES, some ? v + G.vs_off : AT_OUT, rsrc);
-      }
-    }
+  // The loads that belong to step S of N.
+  template <int S, int N>
+  __device__ __forceinline__ void step(const DSV4GCache &C, const CacheGeom &G, const Item &it,
+                                       int wave, int lane) const {
+    constexpr int K0 = (S * F::PER + N - 1) / N, K1 = ((S + 1) * F::PER + N - 1) / N;
+    each<K1 - K0>([&](auto k) { load<K0 + k>(C, G, it, wave, lane); });
   }
 };
 
@@ -434,19 +461,7 @@ __device__ __forceinline__ Bf8 read_vt(uint32_t at, int u, int dt) {
   return __builtin_bit_cast(Bf8, r);
 }
 
-// The order of a product's loop for the scheduler, which else puts each read
-// right in front of the product that waits for it: the LDS reads of the first
-// R steps, then a step's products and the reads of the step R on, in turn.
-constexpr int AT_AHEAD = 6;
-template <int N, int R, int MFMA, int READS>
-__device__ __forceinline__ void sched_steps() {
-  __builtin_amdgcn_sched_group_barrier(0x100, (R < N ? R : N) * READS, 0);
-#pragma unroll
-  for (int s = 0; s < N; ++s) {
-    __builtin_amdgcn_sched_group_barrier(0x008, MFMA, 0);
-    if (s + R < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-  }
-}
+constexpr int AT_AHEAD = 6;  // LDS reads ahead of their product (even)
 
 // An output tile moved between the accumulation registers, where it stays in
 // the loop, and the vector registers that arithmetic needs: one tile at a
@@ -514,6 +529,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
   const uint32_t raw0 = lds0 + F::NTILE * STAGE;  // the ring of codes
   const uint32_t ring0 = FP8 ? raw0 : lds0;
   constexpr int RSTEP = FP8 ? F::RAW : STAGE;
+  constexpr int R = AT_AHEAD;
   if (tid < F::KW) s_odd[tid] = 0;
 
   Place w;
@@ -538,8 +554,9 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       continue;
     }
     it.kvh = w.kvh;
+    one(it);
     const int s0 = w.stage;
-    const int s1 = a.groups ? (int)min((long)it.stages, s0 + w.end - w.at) : it.stages;
+    const int s1 = one(a.groups ? (int)min((long)it.stages, s0 + w.end - w.at) : it.stages);
     if (a.groups) {
       if (s0 == 0 && tid == 0) {
         a.first[1 + (long)w.pair * C.kv_heads + it.kvh] = w.at;
@@ -560,17 +577,16 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     const int r = min(wr0 + lane % 32, it.nrows - 1);
     const int tok = r / a.group, head = it.kvh * a.group + r % a.group;
     const int pos0 = it.len - it.count, pos = pos0 + tok;
-    const int pmin = pos0 + min(wr0, it.nrows - 1) / a.group;
-    const int pmax = pos0 + min(wr0 + 31, it.nrows - 1) / a.group;
+    const int pmin = one(pos0 + min(wr0, it.nrows - 1) / a.group);
+    const int pmax = one(pos0 + min(wr0 + 31, it.nrows - 1) / a.group);
 
     Loader<D, SHARED, FP8, RW> load;
     load.look(C, G, it, s0, wave);
 #pragma unroll
-    for (int i = 0; i < RING - 1; ++i)
-      if (s0 + i < s1) {
-        load.issue(C, G, a, it, s0 + i, ring0 + i * RSTEP, wave, lane);
-        load.look(C, G, it, s0 + i + 1, wave);
-      }
+    for (int i = 0; i < RING - 1; ++i) {
+      load.begin(C, G, a, it, s0 + i, s0 + i < s1, ring0 + i * RSTEP, wave);
+      load.template step<0, 1>(C, G, it, wave, lane);
+    }
 
     // the query rows, once: columns 16 s + 8 h .. + 7 of row lane % 32; a
     // negative scale is taken by their sign
@@ -593,7 +609,8 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         q[s] = __builtin_bit_cast(Bf8, u ^ sign);
       }
     }
-    const float c2 = fabsf(a.scale) * LOG2E;
+    // not 0: a hidden score stays -inf when it is scaled
+    const float c2 = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);
 
     F16v o[NP];
 #pragma unroll
@@ -608,7 +625,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     const uint32_t vat = lds0 + v_at<D>(lane) + 32 * kw * (2 * D) + (SHARED ? 0 : F::KB);
     // tokens that no row sees are not loaded; between these two are those that
     // some row of the workgroup sees and another does not
-    const int shown = pos0 + it.r0 / a.group, hidden = it.hi - 1 - a.window;
+    const int shown = one(pos0 + it.r0 / a.group), hidden = it.hi - 1 - a.window;
 
     if (F::TWICE) {  // the first stage's rows
       wait_loads<0>();
@@ -622,8 +639,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       // ahead) is in LDS for every wave, and every wave is done with the stage
       // before st
       constexpr int AHEAD = F::TWICE ? 1 : 0;
-      if (st + RING - 2 < s1) wait_loads<(RING - 2 - AHEAD) * F::PER>();
-      else wait_loads<0>();
+      wait_loads<(RING - 2 - AHEAD) * F::PER>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -634,10 +650,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         asm volatile("" ::: "memory");
       }
       const int next = st + RING - 1;
-      if (next < s1) {
-        load.issue(C, G, a, it, next, ring0 + (i + RING - 1) % RING * RSTEP, wave, lane);
-        load.look(C, G, it, next + 1, wave);
-      }
+      load.begin(C, G, a, it, next, next < s1, ring0 + (i + RING - 1) % RING * RSTEP, wave);
       const uint32_t here = i % F::NTILE * STAGE;  // the stage's rows
       const int w0 = it.lo + st * TT;                 // the stage's tokens
       const int t0 = w0 + 32 * kw;                    // this wave's 32
@@ -665,26 +678,30 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         for (int k = 0; k < F::KW; ++k) any |= s_odd[k];
         odd = __builtin_amdgcn_readfirstlane(any) ? 1u : 0u;
       }
-      const bool none = !active || t0 > pmax || (a.window && t0 + 31 <= pmin - a.window);
+      // A wave whose rows see nothing of its 32 tokens computes weights of 0: a
+      // branch around the products would have the compiler copy the
+      // accumulators at its ends.
       Bf8 p0, p1;
-      if (!none) {
+      {
         F16v z;
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i] = 0.0f;
         const uint32_t at = kat + here;
-        // reads a few steps ahead of the products that take them
-        constexpr int R = AT_AHEAD;
+        // LDS reads a few steps ahead of the products that take them, and the
+        // next stage's loads between them (issued at once they would hold up
+        // the wave); the order is pinned, since the scheduler puts each read
+        // right in front of its product
         __builtin_amdgcn_sched_barrier(0);
         Bf8 k[R];
 #pragma unroll
         for (int s = 0; s < R && s < KS; ++s) k[s] = read_k<D>(at, s);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[s % R], q[s], z, 0, 0, 0);
-          if (s + R < KS) k[s % R] = read_k<D>(at, s + R);
-        }
-        sched_steps<KS, R, 1, 1>();
         __builtin_amdgcn_sched_barrier(0);
+        each<KS>([&](auto s) {
+          z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[s % R], q[s], z, 0, 0, 0);
+          if constexpr (s + R < KS) k[s % R] = read_k<D>(at, s + R);
+          load.template step<s, 2 * KS>(C, G, it, wave, lane);
+          __builtin_amdgcn_sched_barrier(0);
+        });
         // token of z[i]: t0 + 8 (i / 4) + 4 h + i % 4
         const bool mask = t0 + 31 > pmin || (a.window && t0 <= pmax - a.window);
         if (mask) {
@@ -695,11 +712,12 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
             z[i] = at <= high && at > low ? z[i] : -__builtin_inff();
           }
         }
-        float mx = z[0];
+        float mx = fmaxf(fmaxf(z[0], z[1]), z[2]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, z[i]);
+        for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, z[i]), z[i + 1]);
+        mx = fmaxf(mx, z[15]);
         mx = swap_max(mx);
-        const float mt = mx > -__builtin_inff() ? mx * c2 : -__builtin_inff();
+        const float mt = mx * c2;
         if (__any(mt > m + AT_GROW)) {
           const float M = fmaxf(m, mt);
           const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
@@ -715,18 +733,16 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         }
         const float mu = m > -__builtin_inff() ? m : 0.0f;
         U4 b0, b1;
+        float part[4] = {};
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          float x0 = __builtin_amdgcn_exp2f(fmaf(z[i], c2, -mu));
-          float x1 = __builtin_amdgcn_exp2f(fmaf(z[i + 1], c2, -mu));
-          if (mask) {  // a scale of 0 leaves -inf * 0
-            x0 = z[i] == -__builtin_inff() ? 0.0f : x0;
-            x1 = z[i + 1] == -__builtin_inff() ? 0.0f : x1;
-          }
-          l += x0 + x1;
+          const float x0 = __builtin_amdgcn_exp2f(fmaf(z[i], c2, -mu));
+          const float x1 = __builtin_amdgcn_exp2f(fmaf(z[i + 1], c2, -mu));
+          part[i / 2 % 4] += x0 + x1;
           if (i < 8) b0[i / 2] = pack_bf16(x0, x1);
           else b1[i / 2 - 4] = pack_bf16(x0, x1);
         }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
         p0 = __builtin_bit_cast(Bf8, b0);
         p1 = __builtin_bit_cast(Bf8, b1);
       }
@@ -747,24 +763,23 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         __syncthreads();
         if (tid < F::KW) s_odd[tid] = 0;  // read again two barriers on at the earliest
       }
-      if (!none) {
+      {
         const uint32_t at = vat + here;
-        constexpr int R = AT_AHEAD / 2;
         __builtin_amdgcn_sched_barrier(0);
-        Bf8 v[2 * R];
+        Bf8 v[R];
 #pragma unroll
-        for (int s = 0; s < 2 * R && s < 2 * NP; ++s) v[s] = read_vt<D>(at, s % 2, s / 2);
-#pragma unroll
-        for (int s = 0; s < 2 * NP; ++s) {
-          o[s / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[s % (2 * R)], s % 2 ? p1 : p0,
-                                                             o[s / 2], 0, 0, 0);
-          if (s + 2 * R < 2 * NP)
-            v[s % (2 * R)] = read_vt<D>(at, s % 2, (s + 2 * R) / 2);
-        }
-        sched_steps<2 * NP, 2 * R, 1, 2>();
+        for (int s = 0; s < R && s < KS; ++s) v[s] = read_vt<D>(at, s % 2, s / 2);
         __builtin_amdgcn_sched_barrier(0);
+        each<KS>([&](auto s) {  // two k-steps of each of KS / 2 output tiles
+          o[s / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[s % R], s % 2 ? p1 : p0, o[s / 2],
+                                                             0, 0, 0);
+          if constexpr (s + R < KS) v[s % R] = read_vt<D>(at, s % 2, (s + R) / 2);
+          load.template step<KS + s, 2 * KS>(C, G, it, wave, lane);
+          __builtin_amdgcn_sched_barrier(0);
+        });
       }
     }
+    wait_loads<0>();  // the loads behind the last stage are done with LDS
     l = swap_sum(l);
 
     // the waves that shared the rows: into the first one, through LDS
