@@ -46,6 +46,7 @@ typedef float F16v __attribute__((ext_vector_type(16)));
 typedef short S4 __attribute__((ext_vector_type(4)));
 typedef int I4 __attribute__((ext_vector_type(4)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+typedef uint32_t U2 __attribute__((ext_vector_type(2)));
 // LDS by address
 #define DSV4_LDS(T, at) (*(__attribute__((address_space(3))) T *)(uintptr_t)(at))
 
@@ -94,9 +95,16 @@ struct Cfg {
   // direct loads per wave and stage
   static constexpr int PER = FP8 ? M * (at_max(1, CODES / 4096) + at_max(1, TT / 64))
                                  : STAGE / 4096;
-  // a wave's outputs and its rows' (m, l), handed over when waves share rows
-  static constexpr int PART = 32 * D * 4 + 64 * 8, JOIN = KW > 1 ? RW * PART : 0;
+  // what the other waves of its rows hand a wave at the end: their parts of
+  // its tiles; then every wave's (m, l)
+  static constexpr int NO = at_max(1, NP / KW);  // tiles that a wave ends up with, if any
+  static constexpr int PART = (KW - 1) * NO * 4096, JOIN = KW > 1 ? 4 * PART + 2048 : 0;
   static constexpr int LDS = at_max(NTILE * STAGE + NRAW * RAW, JOIN);
+  // Full tiles are bound by the products, and the next stage's loads go between
+  // them (issued at once they hold up the wave: latent chunk 4.40 -> 3.99 ms);
+  // with fewer rows the memory is the bound and they are issued at once (64
+  // sequences of 4000, grouped heads: 190 us against 215).
+  static constexpr bool SPREAD = RW == 4;
   static constexpr int WGS = LDS <= 80 * 1024 && D <= 128 ? 2 : 1;  // per CU
 };
 
@@ -360,53 +368,50 @@ struct Loader {
   }
 };
 
-// E4M3 codes of a stage as BF16 rows: a code times its power of two is exact
-// in BF16. 16 codes per thread and step.
+// E4M3 codes of a stage as BF16 rows, 8 codes (one chunk of a row) per thread
+// and step: a code times its power of two is exact in BF16. Step p is T = 2048
+// / D rows on, so all addresses are the thread's own XOR and plus constants.
+// Codes that were not loaded are 0, beside whatever scale code the page holds:
+// 255 counts as 254, so that they stay 0.
 template <int D, bool SHARED, int TT>
 __device__ __forceinline__ void convert(uint32_t raw, uint32_t tile, int tid) {
-  constexpr int CODES = TT * D, SCALES = CODES / 64, KB = 2 * CODES;
+  constexpr int CODES = TT * D, SCALES = CODES / 64, T = 2048 / D, P = TT / T, B = P < 4 ? P : 4;
+  static_assert(P >= 1, "a stage is a step or more");
   fresh(tid);
+  const int row = tid * 8 / D;
+  const uint32_t from = raw + 8 * tid, scale = raw + CODES + tid / 8;
+  const uint32_t to = tile + row * (2 * D) + 16 * ((tid * 8 % D / 8) ^ chunk_swizzle<D>(row));
 #pragma unroll
   for (int m = 0; m < (SHARED ? 1 : 2); ++m) {
-    // a batch's reads at once and no branch: each step would else wait for LDS
-    constexpr int P = (CODES + 4095) / 4096, B = P < 4 ? P : 4;
+    const uint32_t fm = m * (CODES + SCALES), tm = m * 2 * CODES;
+    // a batch's reads at once: each step would else wait for LDS
 #pragma unroll
-    for (int p = 0; p < P; p += B) {
-      U4 u[B];
+    for (int p0 = 0; p0 < P; p0 += B) {
+      U2 u[B];
       uint32_t s[B];
 #pragma unroll
       for (int i = 0; i < B; ++i) {
-        const int at = ((p + i) * 256 + tid) * 16 % CODES;  // twice the same where there are fewer
-        u[i] = DSV4_LDS(U4, raw + at);
-        s[i] = DSV4_LDS(uint8_t, raw + CODES + at / 64);
+        u[i] = DSV4_LDS(U2, from + fm + (p0 + i) * 2048);
+        s[i] = DSV4_LDS(uint8_t, scale + fm + (p0 + i) * 32);
       }
 #pragma unroll
       for (int i = 0; i < B; ++i) {
-        const int at = ((p + i) * 256 + tid) * 16 % CODES;
-        const int tl = at / D, ch = at % D / 8, g = chunk_swizzle<D>(tl);
-        // E8M0; codes that were not loaded are 0, beside whatever scale the
-        // page holds
-        uint32_t bits = s[i] << 23;
-        bits = s[i] == 0 ? 0x00400000u : bits;
-        bits = s[i] == 255 ? 0x7FC00000u : bits;
-        bits = (u[i][0] | u[i][1] | u[i][2] | u[i][3]) == 0u ? 0x3F800000u : bits;
-        const float scale = u2f(bits);
-        U4 y[2];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          y[k / 2][2 * (k % 2)] = __builtin_bit_cast(
-              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[i][k], scale, false));
-          y[k / 2][2 * (k % 2) + 1] = __builtin_bit_cast(
-              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[i][k], scale, true));
-        }
-        const uint32_t row = tile + tl * (2 * D);
-        DSV4_LDS(U4, row + 16 * (ch ^ g)) = y[0];
-        DSV4_LDS(U4, row + 16 * ((ch + 1) ^ g)) = y[1];
+        const int p = p0 + i;
+        const float f = u2f(min(s[i], 254u) << 23);
+        auto two = [&](uint32_t w, auto hi) {
+          return __builtin_bit_cast(
+              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, f, decltype(hi)::value));
+        };
+        const std::false_type lo;
+        const std::true_type hi;
+        const U4 y = {two(u[i].x, lo), two(u[i].x, hi), two(u[i].y, lo), two(u[i].y, hi)};
+        // the swizzle of row + p T against the row's own
+        constexpr int X = 16;
+        const uint32_t x = T == 4 ? X * (8 * (p & 1) + (p / 2 & 1)) : T == 8 ? X * (p & 1) : 0;
+        DSV4_LDS(U4, (to ^ x) + tm + p * T * (2 * D)) = y;
       }
       __builtin_amdgcn_sched_barrier(0);  // a batch at a time: registers
     }
-    raw += CODES + SCALES;
-    tile += KB;
   }
 }
 
@@ -521,7 +526,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
   constexpr int TT = F::TT, STAGE = F::STAGE, RING = F::RING, NP = F::NP, KS = D / 16;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[F::LDS];
   __shared__ uint32_t s_odd[F::KW];  // tokens of a stage with something not finite
-  if (*C.status) return;
+  const unsigned bad = *C.status;
   const int tid = threadIdx.x, lane = tid % 64, h = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int rw = wave % RW, kw = wave / RW;
@@ -545,6 +550,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     w.at = 0;
     w.end = 1;
   }
+  if (bad) return;
   // One segment after the other: a run of stages of one item.
   while (w.at < w.end) {
     Item it;
@@ -651,6 +657,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       }
       const int next = st + RING - 1;
       load.begin(C, G, a, it, next, next < s1, ring0 + (i + RING - 1) % RING * RSTEP, wave);
+      if constexpr (!F::SPREAD) load.template step<0, 1>(C, G, it, wave, lane);
       const uint32_t here = i % F::NTILE * STAGE;  // the stage's rows
       const int w0 = it.lo + st * TT;                 // the stage's tokens
       const int t0 = w0 + 32 * kw;                    // this wave's 32
@@ -687,10 +694,9 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i] = 0.0f;
         const uint32_t at = kat + here;
-        // LDS reads a few steps ahead of the products that take them, and the
-        // next stage's loads between them (issued at once they would hold up
-        // the wave); the order is pinned, since the scheduler puts each read
-        // right in front of its product
+        // LDS reads a few steps ahead of the products that take them; the order
+        // is pinned, since the scheduler puts each read right in front of its
+        // product
         __builtin_amdgcn_sched_barrier(0);
         Bf8 k[R];
 #pragma unroll
@@ -699,7 +705,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         each<KS>([&](auto s) {
           z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[s % R], q[s], z, 0, 0, 0);
           if constexpr (s + R < KS) k[s % R] = read_k<D>(at, s + R);
-          load.template step<s, 2 * KS>(C, G, it, wave, lane);
+          if constexpr (F::SPREAD) load.template step<s, 2 * KS>(C, G, it, wave, lane);
           __builtin_amdgcn_sched_barrier(0);
         });
         // token of z[i]: t0 + 8 (i / 4) + 4 h + i % 4
@@ -774,7 +780,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
           o[s / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[s % R], s % 2 ? p1 : p0, o[s / 2],
                                                              0, 0, 0);
           if constexpr (s + R < KS) v[s % R] = read_vt<D>(at, s % 2, (s + R) / 2);
-          load.template step<KS + s, 2 * KS>(C, G, it, wave, lane);
+          if constexpr (F::SPREAD) load.template step<KS + s, 2 * KS>(C, G, it, wave, lane);
           __builtin_amdgcn_sched_barrier(0);
         });
       }
@@ -782,73 +788,89 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     wait_loads<0>();  // the loads behind the last stage are done with LDS
     l = swap_sum(l);
 
-    // the waves that shared the rows: into the first one, through LDS
-    if constexpr (F::KW > 1) {
-      constexpr int PART = F::PART;
-      for (int k = 1; k < F::KW; ++k) {
-        __syncthreads();
-        float4 *x = (float4 *)(lds + rw * PART);
-        float2 *xs = (float2 *)(lds + rw * PART + 32 * D * 4);
-        if (kw == k) {
+    // The waves that shared the rows: a wave hands the others their share of
+    // its output tiles through LDS and takes theirs of its own, NP / KW tiles.
+    constexpr int KW = F::KW, NO = F::NO;
+    float f = 1.0f;                          // its own outputs' factor
+    if constexpr (KW > 1) {
+      float2 *xs = (float2 *)(lds + 4 * F::PART);
+      __syncthreads();
+      each<NP>([&](auto d) {
+        if (d / NO != kw) {  // tile d: to wave d / NO, from this one
+          const F16v y = tile_out(o[d]);
+          const int slot = d % NO * (KW - 1) + (kw > d / NO ? kw - 1 : kw);
+          float4 *x = (float4 *)(lds + (d / NO * RW + rw) * F::PART) + slot * 256;
 #pragma unroll
-          for (int d = 0; d < NP; ++d) {
-            const F16v y = tile_out(o[d]);
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-              x[(4 * d + g) * 64 + lane] =
-                  make_float4(y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          xs[lane] = make_float2(m, l);
+          for (int g = 0; g < 4; ++g)
+            x[g * 64 + lane] =
+                make_float4(y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]);
         }
-        __syncthreads();
-        if (kw == 0) {
-          const float2 s = xs[lane];
-          const float M = fmaxf(m, s.x);
-          const bool any = M > -__builtin_inff();
-          const float f0 = any ? exp2f(m - M) : 1.0f, f1 = any ? exp2f(s.x - M) : 0.0f;
-          l = l * f0 + s.y * f1;
-          m = M;
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      xs[wave * 64 + lane] = make_float2(m, l);
+      __syncthreads();
+      float M = m;
 #pragma unroll
-          for (int d = 0; d < NP; ++d) {
-            F16v y = tile_out(o[d]);
+      for (int k = 0; k < KW; ++k) M = fmaxf(M, xs[(k * RW + rw) * 64 + lane].x);
+      const float mu = M > -__builtin_inff() ? M : 0.0f;
+      f = __builtin_amdgcn_exp2f(m - mu);
+      float fk[KW];
+      l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const float2 s = xs[(k * RW + rw) * 64 + lane];
+        fk[k] = __builtin_amdgcn_exp2f(s.x - mu);
+        l += s.y * fk[k];
+      }
+      m = M;
+      each<NP>([&](auto d) {
+        if (d / NO == kw) {
+          F16v y = tile_out(o[d]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] *= f;
+#pragma unroll
+          for (int k = 0; k < KW; ++k) {
+            if (k == kw) continue;
+            const int slot = d % NO * (KW - 1) + (k > kw ? k - 1 : k);
+            const float4 *x = (const float4 *)(lds + wave * F::PART) + slot * 256;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const float4 p = x[(4 * d + g) * 64 + lane];
-              y[4 * g] = y[4 * g] * f0 + p.x * f1;
-              y[4 * g + 1] = y[4 * g + 1] * f0 + p.y * f1;
-              y[4 * g + 2] = y[4 * g + 2] * f0 + p.z * f1;
-              y[4 * g + 3] = y[4 * g + 3] * f0 + p.w * f1;
+              const float4 p = x[g * 64 + lane];
+              y[4 * g] += p.x * fk[k];
+              y[4 * g + 1] += p.y * fk[k];
+              y[4 * g + 2] += p.z * fk[k];
+              y[4 * g + 3] += p.w * fk[k];
             }
-            tile_in(o[d], y);
           }
+          tile_in(o[d], y);
         }
-      }
+      });
     }
-    if (kw == 0 && active && wr0 + lane % 32 < it.nrows) {
+    if (active && wr0 + lane % 32 < it.nrows) {
       if (s0 > 0 || s1 < it.stages) {
         const size_t slot = 2 * (size_t)blockIdx.x + (s0 == 0);  // the run's last item, or its first
         float4 *to = (float4 *)(a.part + (slot * F::ROWS + 32 * rw) * D);
+        each<NP>([&](auto d) {
+          if (KW == 1 || d / NO == kw) {
+            const F16v y = tile_out(o[d]);
 #pragma unroll
-        for (int d = 0; d < NP; ++d) {
-          const F16v y = tile_out(o[d]);
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            to[(4 * d + g) * 64 + lane] =
-                make_float4(y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]);
+            for (int g = 0; g < 4; ++g)
+              to[(4 * d + g) * 64 + lane] =
+                  make_float4(y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]);
+          }
           __builtin_amdgcn_sched_barrier(0);
-        }
-        if (h == 0) a.stat[slot * F::ROWS + 32 * rw + lane] = make_float2(m, l);
+        });
+        if (kw == 0 && h == 0) a.stat[slot * F::ROWS + 32 * rw + lane] = make_float2(m, l);
       } else {
         float lse;
-        const float f = finish_row(a, head, m, l, &lse);
+        const float r = finish_row(a, head, m, l, &lse);
         const size_t row = (size_t)(it.start + tok);
-#pragma unroll
-        for (int d = 0; d < NP; ++d) {
-          store_tile<D>(a, row * a.out_stride + (size_t)head * D, d, h, tile_out(o[d]), f);
+        each<NP>([&](auto d) {
+          if (KW == 1 || d / NO == kw)
+            store_tile<D>(a, row * a.out_stride + (size_t)head * D, d, h, tile_out(o[d]), r);
           __builtin_amdgcn_sched_barrier(0);
-        }
-        if (a.lse && h == 0) a.lse[row * a.heads + head] = lse;
+        });
+        if (a.lse && kw == 0 && h == 0) a.lse[row * a.heads + head] = lse;
       }
     }
     if (!a.groups) return;
@@ -856,55 +878,107 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
   }
 }
 
-// Joins the parts of every item that several workgroups shared: one wave per
-// output tile of a row wave.
+// Joins the parts of every item that several workgroups shared: a workgroup
+// per output tile of a row wave, whose four waves take every fourth part.
 template <int D, int RW>
 __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   constexpr int TT = 32 * (4 / RW), ROWS = 32 * RW, NP = D / 32;
-  if (*C.status) return;
+  __shared__ float4 s_o[3][4][64];
+  __shared__ float2 s_l[3][64];
+  const unsigned bad = *C.status;
   const int lane = threadIdx.x % 64, h = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  int id = blockIdx.x * 4 + wave;
+  int id = blockIdx.x;
   const int d = id % NP;
   id /= NP;
   const int rw = id % RW;
   id /= RW;  // (sequence, tile), kv head
   const int kvh = id % C.kv_heads, pair = id / C.kv_heads;
-  if (pair >= a.n_seqs * a.tiles) return;
-  Item it;
-  if (!attn_item<ROWS, TT>(C, a, pair / a.tiles, pair % a.tiles, it)) return;
   const long total = a.first[0], at = a.first[1 + id];
+  Item it;
+  if (bad || !attn_item<ROWS, TT>(C, a, pair / a.tiles, pair % a.tiles, it)) return;
   const int groups = shared_groups(a, total);
   const int w0 = share_of(total, groups, at), w1 = share_of(total, groups, at + it.stages - 1);
+  if (w0 == w1) return;
   const int r = it.r0 + 32 * rw + lane % 32;
-  if (w0 == w1 || r >= it.nrows) return;
+  const bool live = r < it.nrows;  // parts hold such rows only
   // the first workgroup's part is its run's last, the others' their first
   auto slot = [&](int w) { return (2 * (size_t)w + (w == w0)) * ROWS + 32 * rw; };
   float m = -__builtin_inff(), l = 0.0f;
-#pragma unroll 4
-  for (int w = w0; w <= w1; ++w) m = fmaxf(m, a.stat[slot(w) + lane % 32].x);
-  const float mu = m > -__builtin_inff() ? m : 0.0f;
   F16v o;
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = 0.0f;
-#pragma unroll 4
-  for (int w = w0; w <= w1; ++w) {
-    const float2 s = a.stat[slot(w) + lane % 32];
-    const float f = __builtin_amdgcn_exp2f(s.x - mu);
-    l += s.y * f;
-    const float4 *from = (const float4 *)(a.part + slot(w) * D);
+  constexpr int U = 4;  // parts in flight
+  for (int w = w0 + wave; w <= w1; w += 4 * U) {
+    float2 s[U];
+    float4 x[U][4];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      s[k] = make_float2(-__builtin_inff(), 0.0f);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x[k][g] = make_float4(0, 0, 0, 0);
+      if (live && w + 4 * k <= w1) {
+        const size_t at = slot(w + 4 * k);
+        s[k] = a.stat[at + lane % 32];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) x[k][g] = ((const float4 *)(a.part + at * D))[(4 * d + g) * 64 + lane];
+      }
+    }
+    float M = m;
+#pragma unroll
+    for (int k = 0; k < U; ++k) M = fmaxf(M, s[k].x);
+    const float mu = M > -__builtin_inff() ? M : 0.0f;
+    const float f = __builtin_amdgcn_exp2f(m - mu);
+    m = M;
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] *= f;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float p = __builtin_amdgcn_exp2f(s[k].x - mu);
+      l += s[k].y * p;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        o[4 * g] += x[k][g].x * p;
+        o[4 * g + 1] += x[k][g].y * p;
+        o[4 * g + 2] += x[k][g].z * p;
+        o[4 * g + 3] += x[k][g].w * p;
+      }
+    }
+  }
+  if (wave) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      s_o[wave - 1][g][lane] = make_float4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
+    s_l[wave - 1][lane] = make_float2(m, l);
+  }
+  __syncthreads();
+  if (wave || !live) return;
+  float M = m;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) M = fmaxf(M, s_l[k][lane].x);
+  const float mu = M > -__builtin_inff() ? M : 0.0f;
+  const float f0 = __builtin_amdgcn_exp2f(m - mu);
+  l *= f0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] *= f0;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float2 s = s_l[k][lane];
+    const float p = __builtin_amdgcn_exp2f(s.x - mu);
+    l += s.y * p;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 x = from[(4 * d + g) * 64 + lane];
-      o[4 * g] += x.x * f;
-      o[4 * g + 1] += x.y * f;
-      o[4 * g + 2] += x.z * f;
-      o[4 * g + 3] += x.w * f;
+      const float4 x = s_o[k][g][lane];
+      o[4 * g] += x.x * p;
+      o[4 * g + 1] += x.y * p;
+      o[4 * g + 2] += x.z * p;
+      o[4 * g + 3] += x.w * p;
     }
   }
   const int tok = r / a.group, head = kvh * a.group + r % a.group;
   float lse;
-  const float f = finish_row(a, head, m, l, &lse);
+  const float f = finish_row(a, head, M, l, &lse);
   const size_t row = (size_t)(it.start + tok);
   store_tile<D>(a, row * a.out_stride + (size_t)head * D, d, h, o, f);
   if (a.lse && h == 0 && d == 0) a.lse[row * a.heads + head] = lse;
@@ -953,7 +1027,7 @@ static void attn_launch(const DSV4GCache &C, const CacheGeom &G, const AttnArgs 
     hipLaunchKernelGGL((k_attn<D, SHARED, FP8, RW>), dim3((unsigned)(a.groups ? a.groups : items)),
                        dim3(256), 0, st, C, G, a);
     if (a.groups)
-      hipLaunchKernelGGL((k_attn_join<D, RW>), dim3((unsigned)((items * RW * (D / 32) + 3) / 4)),
+      hipLaunchKernelGGL((k_attn_join<D, RW>), dim3((unsigned)(items * RW * (D / 32))),
                          dim3(256), 0, st, C, a);
   }
 }
