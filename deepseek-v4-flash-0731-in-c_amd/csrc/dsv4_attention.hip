@@ -100,11 +100,10 @@ struct Cfg {
   static constexpr int NO = at_max(1, NP / KW);  // tiles that a wave ends up with, if any
   static constexpr int PART = (KW - 1) * NO * 4096, JOIN = KW > 1 ? 4 * PART + 2048 : 0;
   static constexpr int LDS = at_max(NTILE * STAGE + NRAW * RAW, JOIN);
-  // Full tiles are bound by the products, and the next stage's loads go between
-  // them (issued at once they hold up the wave: latent chunk 4.40 -> 3.99 ms);
-  // with fewer rows the memory is the bound and they are issued at once (64
-  // sequences of 4000, grouped heads: 190 us against 215).
-  static constexpr bool SPREAD = RW == 4;
+  // The next stage's loads go between the products (issued at once they hold up
+  // the wave): of a full tile, bound by the products, between all of them;
+  // with fewer rows, bound by the memory, between those of the first half.
+  static constexpr int OVER = (RW == 4 ? 2 : 1) * (D / 16);
   static constexpr int WGS = LDS <= 80 * 1024 && D <= 128 ? 2 : 1;  // per CU
 };
 
@@ -185,11 +184,13 @@ __device__ __forceinline__ int share_of(long total, int groups, long at) {
 struct Place {
   long at, end, total;
   int pair, kvh, stage;
+  Item it;  // of the first pair
 };
 template <int ROWS, int TT>
 __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &a, Place &p) {
   __shared__ long s_sum[4];
   __shared__ int s_at[3];
+  __shared__ Item s_item;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   const int pairs = a.n_seqs * a.tiles, per = (pairs + 255) / 256;
   const int j0 = min(pairs, tid * per), j1 = min(pairs, j0 + per);
@@ -226,6 +227,7 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
           s_at[0] = j;
           s_at[1] = (int)((p.at - before) / it.stages);
           s_at[2] = (int)((p.at - before) % it.stages);
+          s_item = it;
           break;
         }
         before += all;
@@ -234,6 +236,7 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
   p.pair = __builtin_amdgcn_readfirstlane(s_at[0]);
   p.kvh = __builtin_amdgcn_readfirstlane(s_at[1]);
   p.stage = __builtin_amdgcn_readfirstlane(s_at[2]);
+  p.it = s_item;
 }
 
 // A value whose uses are computed again each time: addresses derived from it
@@ -381,38 +384,39 @@ __device__ __forceinline__ void convert(uint32_t raw, uint32_t tile, int tid) {
   const int row = tid * 8 / D;
   const uint32_t from = raw + 8 * tid, scale = raw + CODES + tid / 8;
   const uint32_t to = tile + row * (2 * D) + 16 * ((tid * 8 % D / 8) ^ chunk_swizzle<D>(row));
+  constexpr int M = SHARED ? 1 : 2, N = M * P / B;  // batches
+  U2 u[2][B];
+  uint32_t s[2][B];
+  auto read = [&](auto n) {
+    constexpr uint32_t fm = n * B / P * (CODES + SCALES), p0 = n * B % P;
 #pragma unroll
-  for (int m = 0; m < (SHARED ? 1 : 2); ++m) {
-    const uint32_t fm = m * (CODES + SCALES), tm = m * 2 * CODES;
-    // a batch's reads at once: each step would else wait for LDS
-#pragma unroll
-    for (int p0 = 0; p0 < P; p0 += B) {
-      U2 u[B];
-      uint32_t s[B];
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        u[i] = DSV4_LDS(U2, from + fm + (p0 + i) * 2048);
-        s[i] = DSV4_LDS(uint8_t, scale + fm + (p0 + i) * 32);
-      }
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        const int p = p0 + i;
-        const float f = u2f(min(s[i], 254u) << 23);
-        auto two = [&](uint32_t w, auto hi) {
-          return __builtin_bit_cast(
-              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, f, decltype(hi)::value));
-        };
-        const std::false_type lo;
-        const std::true_type hi;
-        const U4 y = {two(u[i].x, lo), two(u[i].x, hi), two(u[i].y, lo), two(u[i].y, hi)};
-        // the swizzle of row + p T against the row's own
-        constexpr int X = 16;
-        const uint32_t x = T == 4 ? X * (8 * (p & 1) + (p / 2 & 1)) : T == 8 ? X * (p & 1) : 0;
-        DSV4_LDS(U4, (to ^ x) + tm + p * T * (2 * D)) = y;
-      }
-      __builtin_amdgcn_sched_barrier(0);  // a batch at a time: registers
+    for (int i = 0; i < B; ++i) {
+      u[n % 2][i] = DSV4_LDS(U2, from + fm + (p0 + i) * 2048);
+      s[n % 2][i] = DSV4_LDS(uint8_t, scale + fm + (p0 + i) * 32);
     }
-  }
+  };
+  read(std::integral_constant<int, 0>{});
+  each<N>([&](auto n) {  // the next batch's reads under this one's arithmetic
+    if constexpr (n + 1 < N) read(std::integral_constant<int, n + 1>{});
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int p = n * B % P + i;
+      const float f = u2f(min(s[n % 2][i], 254u) << 23);
+      auto two = [&](uint32_t w, auto hi) {
+        return __builtin_bit_cast(
+            uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, f, decltype(hi)::value));
+      };
+      const std::false_type lo;
+      const std::true_type hi;
+      const U2 w = u[n % 2][i];
+      const U4 y = {two(w.x, lo), two(w.x, hi), two(w.y, lo), two(w.y, hi)};
+      // the swizzle of row + p T against the row's own
+      const uint32_t x = T == 4 ? 16 * (8 * (p & 1) + (p / 2 & 1)) : T == 8 ? 16 * (p & 1) : 0;
+      DSV4_LDS(U4, (to ^ x) + n * B / P * 2 * CODES + p * T * (2 * D)) = y;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  });
 }
 
 __device__ __forceinline__ float swap_max(float v) {  // with the other half of the wave
@@ -552,9 +556,11 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
   }
   if (bad) return;
   // One segment after the other: a run of stages of one item.
-  while (w.at < w.end) {
+  for (bool first = true; w.at < w.end; first = false) {
     Item it;
-    if (!attn_item<F::ROWS, TT>(C, a, w.pair / a.tiles, w.pair % a.tiles, it)) {
+    if (first && a.groups) {
+      it = w.it;  // looked up already
+    } else if (!attn_item<F::ROWS, TT>(C, a, w.pair / a.tiles, w.pair % a.tiles, it)) {
       if (!a.groups) return;
       ++w.pair;  // no rows here
       continue;
@@ -609,8 +615,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
           u = U4{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w), pack_bf16(y.x, y.y),
                  pack_bf16(y.z, y.w)};
         } else {
-          const uint4 x = *(const uint4 *)((const uint16_t *)a.q + at + 16 * s);
-          u = U4{x.x, x.y, x.z, x.w};
+          u = *(const U4 *)((const uint16_t *)a.q + at + 16 * s);
         }
         q[s] = __builtin_bit_cast(Bf8, u ^ sign);
       }
@@ -657,7 +662,6 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       }
       const int next = st + RING - 1;
       load.begin(C, G, a, it, next, next < s1, ring0 + (i + RING - 1) % RING * RSTEP, wave);
-      if constexpr (!F::SPREAD) load.template step<0, 1>(C, G, it, wave, lane);
       const uint32_t here = i % F::NTILE * STAGE;  // the stage's rows
       const int w0 = it.lo + st * TT;                 // the stage's tokens
       const int t0 = w0 + 32 * kw;                    // this wave's 32
@@ -705,7 +709,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         each<KS>([&](auto s) {
           z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[s % R], q[s], z, 0, 0, 0);
           if constexpr (s + R < KS) k[s % R] = read_k<D>(at, s + R);
-          if constexpr (F::SPREAD) load.template step<s, 2 * KS>(C, G, it, wave, lane);
+          load.template step<s, F::OVER>(C, G, it, wave, lane);
           __builtin_amdgcn_sched_barrier(0);
         });
         // token of z[i]: t0 + 8 (i / 4) + 4 h + i % 4
@@ -774,13 +778,13 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         __builtin_amdgcn_sched_barrier(0);
         Bf8 v[R];
 #pragma unroll
-        for (int s = 0; s < R && s < KS; ++s) v[s] = read_vt<D>(at, s % 2, s / 2);
+        for (int s = 0; s < R && s < KS; ++s) v[s] = read_vt<D>(at, s / NP, s % NP);
         __builtin_amdgcn_sched_barrier(0);
-        each<KS>([&](auto s) {  // two k-steps of each of KS / 2 output tiles
-          o[s / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[s % R], s % 2 ? p1 : p0, o[s / 2],
-                                                             0, 0, 0);
-          if constexpr (s + R < KS) v[s % R] = read_vt<D>(at, s % 2, (s + R) / 2);
-          if constexpr (F::SPREAD) load.template step<KS + s, 2 * KS>(C, G, it, wave, lane);
+        each<KS>([&](auto s) {  // each output tile's first k-step, then each one's second
+          o[s % NP] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[s % R], s < NP ? p0 : p1,
+                                                              o[s % NP], 0, 0, 0);
+          if constexpr (s + R < KS) v[s % R] = read_vt<D>(at, (s + R) / NP, (s + R) % NP);
+          if constexpr (F::OVER > KS) load.template step<KS + s, F::OVER>(C, G, it, wave, lane);
           __builtin_amdgcn_sched_barrier(0);
         });
       }
