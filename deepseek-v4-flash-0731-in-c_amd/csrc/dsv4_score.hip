@@ -2,26 +2,40 @@
 // the top alternatives, from rows of logits (dsv4g_logprobs, beside the greedy
 // pick). No counterpart in the reference.
 //
-// One pass over the logits. With z = scale * logit, every thread keeps the
-// running maximum m, s = sum e^(z - m) and t = sum e^(z - m) (z - m) of what it
-// has seen; two such triples join as
-//   m' = max(m1, m2),  f = e^(m1 - m'),
-//   s' = f s1 + .. ,   t' = f (t1 + (m1 - m') s1) + ..
-// and at the end lse = m + log s, entropy = log s - t / s. All in fp32, whose
-// sums run over at most a few hundred terms per thread before they are joined
-// pairwise.
+// One pass over the logits. With z = scale * logit and L = log2 e, every thread
+// keeps the running maximum m of its z and, with M = fl(m L),
+//   s = sum 2^(z L - M),  t = sum 2^(z L - M) (z L - M)
+// (one fma and the hardware's 2^x per logit); two such triples join as
+//   m' = max(m1, m2),  f = 2^(M1 - M'),
+//   s' = f s1 + ..,    t' = f (t1 + (M1 - M') s1) + ..
+// and at the end, with d = m L - M, the rounding of M, exactly by an fma,
+//   lse - m = ln s - d ln 2,  entropy = ln s - (t / s) ln 2.
+// All in fp32, whose sums run over at most a few hundred terms per thread
+// before they are joined pairwise. A maximum below SC_LOW counts as SC_LOW (a
+// row of nothing but a mask of the type's lowest value is even); -inf, a token
+// that cannot be taken, weighs nothing.
 //
 // The top k are kept per wave, one key per lane in descending order (k <= 64):
 // (value as an ordered whole number, ~index), so keys are unique and equal
 // values go to the lower index. A wave's indices only grow, so a value enters
-// if it is strictly above the k-th one kept: a float comparison per logit, and
-// an insertion (a ballot and one shift over the lanes) for the few that pass.
-// Where many pass (the first tile; rows in ascending order), the bar is first
-// raised to the k-th largest of the 64 lanes' own maxima, found bit by bit
-// with ballots: at least k of the tile's values reach it.
+// if it is strictly above the k-th one kept. It must also reach the least of the
+// four waves' (k / 4)-th values: k values of the row do. A comparison with the
+// tile's maximum decides whether the tile is looked through at all. What passes
+// is listed in LDS, 64 at a time, and inserted (a ballot and one shift over the
+// lanes) or, above SC_FEW of them, sorted and merged. In the first tile the bar
+// is the k-th largest of the 64 lanes' own maxima, found bit by bit with ballots:
+// at least k of the tile's values reach it. Two sorted lists merge in 6 steps:
+// the larger of a[i] and b[63 - i] is the upper half of both, a bitonic sequence.
 //
-// Bound: HBM. Rows are cut into segments so that a launch has about 2048
-// workgroups where there are fewer rows; a second launch joins the segments.
+// Bound: HBM for fp32 rows (2048 rows of 129280: 196 us, 5.4 TB/s), the vector
+// units for BF16 ones, with half the bytes per value (156 us, 3.4 TB/s: 8.5
+// instructions a value, one of them 2^x at a quarter of the rate). k = 8 adds 18
+// and 58 us: a wave looks through its first tiles and then ever fewer. Fewer
+// registers for it (six waves per SIMD in place of five) cost 10%: the sort's
+// lane masks are then computed at each use.
+// Rows are cut into segments until a launch has about 2048 workgroups, what the
+// chip holds at once; a second launch joins them (64 rows 13 us, one row 17 us,
+// against 278 and 303 us in library calls).
 #include "dsv4_device.h"
 #include "dsv4_gpu_internal.h"
 
@@ -31,7 +45,9 @@ constexpr int SC_T = 256;              // threads
 constexpr int SC_E = 16;               // logits per thread and tile
 constexpr int SC_TILE = SC_T * SC_E;   // logits per tile: segments are multiples
 constexpr int SC_MAX_SEG = 64;         // segments of a row (one lane each when joined)
-constexpr float SC_LOW = -3.4028235e38f;  // a maximum that e^(-inf - m) survives
+constexpr float SC_LOW = -0x1p126f;    // least z in the sums (times L it is exact)
+constexpr float SC_L = 1.4426950408889634f, SC_LN2 = 0.6931471805599453f;
+constexpr int SC_FEW = 6;              // values that are inserted one by one
 
 // Stats of part of a row, as the segments' launch leaves them.
 struct ScorePart {
@@ -61,16 +77,86 @@ __device__ __forceinline__ float unordered(uint32_t o) {
   return u2f((o >> 31) ? o ^ 0x80000000u : ~o);
 }
 
+__device__ __forceinline__ float score_ref(float m) { return fmaxf(m, SC_LOW) * SC_L; }
+// f of a sum referred to M1, now to M, and its t.
+__device__ __forceinline__ float score_shift(float M1, float M, float s, float &t) {
+  const float f = __builtin_amdgcn_exp2f(M1 - M);
+  t = f * (t + fmaxf(M1 - M, -300.0f) * s);  // f is 0 below: no 0 * inf
+  return f * s;
+}
 __device__ __forceinline__ void score_join(float &m, float &s, float &t, float m2, float s2,
                                            float t2) {
-  const float M = fmaxf(m, m2), f1 = __expf(m - M), f2 = __expf(m2 - M);
-  // below -200 the factor is 0: no 0 * -inf
-  t = f1 * (t + fmaxf(m - M, -200.0f) * s) + f2 * (t2 + fmaxf(m2 - M, -200.0f) * s2);
-  s = f1 * s + f2 * s2;
-  m = M;
+  const float mm = fmaxf(m, m2), M = score_ref(mm);
+  s = score_shift(score_ref(m), M, s, t) + score_shift(score_ref(m2), M, s2, t2);
+  t += t2;
+  m = mm;
 }
 
-// The k largest keys, one per lane, descending (0: none).
+// Another lane's key, and the exchange step of a sort: lanes with bit X set
+// keep the smaller (up: the larger) of the two.
+template <int X>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  const int lane = threadIdx.x;
+  if (X == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
+  if (X == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? r[0] : r[1];
+  }
+  if (X == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);  // row_ror:8
+  if (X == 4) {
+    const uint32_t u = __builtin_amdgcn_update_dpp(0, v, 0x104, 0xf, 0x5, false);  // row_shl:4
+    return __builtin_amdgcn_update_dpp(u, v, 0x114, 0xf, 0xa, false);              // row_shr:4
+  }
+  return __builtin_amdgcn_update_dpp(0, v, X == 2 ? 0x4E : 0xB1, 0xf, 0xf, false);  // quad_perm
+}
+template <int X>
+__device__ __forceinline__ uint64_t exchange(uint64_t key, bool up) {
+  const uint64_t other = ((uint64_t)lane_xor<X>((uint32_t)(key >> 32)) << 32) |
+                         lane_xor<X>((uint32_t)key);
+  const bool small = ((threadIdx.x & X) != 0) != up;
+  return (other < key) == small ? other : key;
+}
+// A bitonic sequence over the lanes into descending order.
+__device__ __forceinline__ uint64_t bitonic_down(uint64_t key) {
+  key = exchange<32>(key, false);
+  key = exchange<16>(key, false);
+  key = exchange<8>(key, false);
+  key = exchange<4>(key, false);
+  key = exchange<2>(key, false);
+  return exchange<1>(key, false);
+}
+// Any keys into ascending order.
+__device__ __forceinline__ uint64_t sort_up(uint64_t key) {
+  const int l = threadIdx.x % 64;
+  auto up = [&](int k) { return (l & k) == 0; };  // runs of k: up and down in turn
+  key = exchange<1>(key, up(2));
+  key = exchange<2>(key, up(4));
+  key = exchange<1>(key, up(4));
+  key = exchange<4>(key, up(8));
+  key = exchange<2>(key, up(8));
+  key = exchange<1>(key, up(8));
+  key = exchange<8>(key, up(16));
+  key = exchange<4>(key, up(16));
+  key = exchange<2>(key, up(16));
+  key = exchange<1>(key, up(16));
+  key = exchange<16>(key, up(32));
+  key = exchange<8>(key, up(32));
+  key = exchange<4>(key, up(32));
+  key = exchange<2>(key, up(32));
+  key = exchange<1>(key, up(32));
+  key = exchange<32>(key, true);
+  key = exchange<16>(key, true);
+  key = exchange<8>(key, true);
+  key = exchange<4>(key, true);
+  key = exchange<2>(key, true);
+  return exchange<1>(key, true);
+}
+
+// The k largest keys, one per lane, descending (0: none); lanes from k on hold
+// what else they happen to.
 struct TopList {
   uint64_t key;
   float bar;   // value of the k-th one
@@ -91,7 +177,10 @@ struct TopList {
                                                     false);
     const uint64_t below = ((uint64_t)hi << 32) | lo;
     key = lane < pos ? key : lane == pos ? x : below;
-    settle(k);
+  }
+  // other: ascending over the lanes
+  __device__ __forceinline__ void merge_up(uint64_t other) {
+    key = bitonic_down(other > key ? other : key);
   }
   __device__ __forceinline__ void settle(int k) {
     const uint32_t h = __builtin_amdgcn_readlane((uint32_t)(key >> 32), k - 1);
@@ -100,14 +189,6 @@ struct TopList {
     bar = unordered(h);
   }
 };
-
-// x into the list of the wave, for a wave's descending keys x(0), x(1), ..:
-// false at the first that does not enter (nor do those behind it).
-__device__ __forceinline__ bool top_offer(TopList &top, uint64_t x, int k) {
-  if (!x || __popcll(__ballot(top.key > x)) >= k) return false;
-  top.insert(x, k);
-  return true;
-}
 
 // 16 logits of a thread from row offset i0 + the thread's places: 16-byte
 // loads where a whole tile is inside the row, guarded single ones at its end.
@@ -152,20 +233,23 @@ struct Tile {
 __device__ __forceinline__ void score_write(const ScoreArgs &a, int row, float m, float s,
                                             float t, int above, uint64_t key, bool have_token,
                                             float zt) {
-  const float ls = logf(s);  // z - lse as (z - m) - log s: m may be large
+  // z - lse as (z - m) - (lse - m): m may be large
+  const float mc = fmaxf(m, SC_LOW);
+  const float ls = logf(s) - fmaf(mc, SC_L, -score_ref(m)) * SC_LN2;
+  const bool fine = s > 0.0f && m > -__builtin_inff();
   const int lane = threadIdx.x % 64;
   const float nan = __builtin_nanf("");
   if (lane == 0) {
-    if (a.logprob) a.logprob[row] = have_token && s > 0.0f ? (zt - m) - ls : nan;
-    if (a.rank) a.rank[row] = have_token && s > 0.0f ? above : -1;
-    if (a.entropy) a.entropy[row] = s > 0.0f ? ls - t / s : nan;
+    if (a.logprob) a.logprob[row] = have_token && fine ? (zt - m) - ls : nan;
+    if (a.rank) a.rank[row] = have_token && fine ? above : -1;
+    if (a.entropy) a.entropy[row] = fine ? logf(s) - t / s * SC_LN2 : nan;
   }
   if (lane < a.k) {
     const size_t o = (size_t)row * a.k + lane;
     const int id = key ? (int)(0xFFFFFFFFu - (uint32_t)key) : -1;
     if (a.top_id) a.top_id[o] = id;
     if (a.top_logprob)
-      a.top_logprob[o] = id >= 0 && s > 0.0f ? (unordered((uint32_t)(key >> 32)) - m) - ls : nan;
+      a.top_logprob[o] = id >= 0 && fine ? (unordered((uint32_t)(key >> 32)) - m) - ls : nan;
   }
 }
 
@@ -175,6 +259,7 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
   __shared__ float s_m[4], s_s[4], s_t[4];
   __shared__ int s_above[4];
   __shared__ uint64_t s_key[TOP ? 4 * 64 : 1];
+  __shared__ volatile float s_bar[4];  // each wave's (k / 4)-th value so far
   const int tid = threadIdx.x, lane = tid % 64;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int row = SPLIT ? blockIdx.x / a.nseg : blockIdx.x;
@@ -190,8 +275,12 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
     const T e = l[token];
     zt = fmaf(sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16), a.scale, 0.0f);
   }
-  float m = SC_LOW, s = 0.0f, t = 0.0f;
-  int above = 0;
+  if (TOP) {
+    if (tid < 4) s_bar[tid] = -__builtin_inff();
+    __syncthreads();
+  }
+  float m = -__builtin_inff(), M = score_ref(m), s = 0.0f, t = 0.0f;
+  int above = 0;  // the wave's
   TopList top;
   top.init();
   for (int at = c0; at < end; at += SC_TILE) {
@@ -199,82 +288,104 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
 #pragma unroll
     for (int j = 0; j < SC_E; ++j) z[j] = tile.value(j, a.scale);
     if (at + SC_TILE < end) tile.load(l, at + SC_TILE, end);  // in flight while this one is summed
-    float mt = z[0];
+    float mt = fmaxf(z[0], z[1]);
 #pragma unroll
-    for (int j = 1; j < SC_E; ++j) mt = fmaxf(mt, z[j]);
+    for (int j = 2; j < SC_E; j += 2) mt = fmaxf(fmaxf(mt, z[j]), z[j + 1]);
     if (mt > m) {
-      const float f = __expf(m - mt);
-      t = f * (t + fmaxf(m - mt, -200.0f) * s);
-      s *= f;
       m = mt;
+      const float N = score_ref(m);
+      s = score_shift(M, N, s, t);
+      M = N;
     }
-    const int ti = token - at;
+    if (m >= SC_LOW) {
 #pragma unroll
-    for (int j = 0; j < SC_E; ++j) {
-      const float d = z[j] - m, e = __expf(d);
-      s += e;
-      t = fmaf(e, fmaxf(d, -200.0f), t);  // e is 0 there: no 0 * -inf
-      above += z[j] > zt || (z[j] == zt && tile.place(j) < ti);
+      for (int j = 0; j < SC_E; ++j) {
+        const float d = fmaf(z[j], SC_L, -M), e = __builtin_amdgcn_exp2f(d);
+        s += e;
+        t = fmaf(e, __builtin_amdgcn_fmed3f(d, -300.0f, 300.0f), t);  // no 0 * inf
+      }
+    } else {  // nothing above the least value yet: those there weigh 1, -inf nothing
+#pragma unroll
+      for (int j = 0; j < SC_E; ++j)
+        s += z[j] > -__builtin_inff() ? 1.0f : z[j] == z[j] ? 0.0f : z[j];
     }
-    if (TOP) {
-      uint32_t least = 0;  // smallest ordered value that enters
-      int many = 0;
-      if (top.full) {
+    // rank: equal values count where they come first (few tiles reach the token's)
+    if (__any(mt >= zt)) {
 #pragma unroll
-        for (int j = 0; j < SC_E; ++j) many += __popcll(__ballot(z[j] > top.bar));
-        if (many) least = ordered(top.bar) + 1;
-      }
-      if (!top.full || many > 2 * a.k) {
-        // the k-th largest of the lanes' maxima, bit by bit; places behind
-        // the row's end rank below every value
-        uint32_t mine = 0;
+      for (int j = 0; j < SC_E; ++j)
+        above += __popcll(__ballot(z[j] > zt || (z[j] == zt && at + tile.place(j) < token)));
+    }
+    if constexpr (TOP) {
+      // Four waves' (k / 4)-th values or better are k values of the row: nothing
+      // below the least of them is among its k.
+      const float least4 = fminf(fminf(s_bar[0], s_bar[1]), fminf(s_bar[2], s_bar[3]));
+      if (!top.full || __any(mt > top.bar && mt >= least4)) {
+        float enters;  // the smallest value that does
+        if (top.full) {
+          enters = fmaxf(unordered(ordered(top.bar) + 1), least4);
+        } else {
+          // the k-th largest of the lanes' maxima, bit by bit. NaN counts as
+          // -inf; places behind the row's end as NaN, which never enters.
+          uint32_t mine = 0, least = 0;
 #pragma unroll
-        for (int j = 0; j < SC_E; ++j)
-          if (at + tile.place(j) < end) mine = max(mine, ordered(z[j]));
-        uint32_t x = 0;
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-          if (__popcll(__ballot(mine >= (x | bit))) >= a.k) x |= bit;
-        least = max(least, x);
-        many = 1;
-      }
-      if (many) {
-#pragma unroll
-        for (int j = 0; j < SC_E; ++j) {
-          const uint32_t o = ordered(z[j]);
-          uint64_t who = __ballot(o >= least && at + tile.place(j) < end);
-          while (who) {
-            const int b = __builtin_ctzll(who);
-            who &= who - 1;
-            const uint32_t ob = __builtin_amdgcn_readlane(o, b);
-            const uint32_t ib = at + (j / Tile<T>::V) * (SC_T * Tile<T>::V) +
-                                Tile<T>::V * (64 * wave + b) + j % Tile<T>::V;
-            top.insert(((uint64_t)ob << 32) | (0xFFFFFFFFu - ib), a.k);
+          for (int j = 0; j < SC_E; ++j) {
+            const bool in = at + tile.place(j) < end;
+            const uint32_t o = ordered(z[j]);
+            z[j] = in ? unordered(o) : __builtin_nanf("");
+            mine = in ? max(mine, o) : mine;
           }
+          for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+            if (__popcll(__ballot(mine >= (least | bit))) >= a.k) least |= bit;
+          enters = least ? unordered(least) : -__builtin_inff();
         }
+        // 64 candidates at a time, through LDS
+        uint64_t *cand = s_key + 64 * wave;
+        int total = 0;
+        for (int from = 0; from == 0 || from < total; from += 64) {
+          total = 0;
+#pragma unroll
+          for (int j = 0; j < SC_E; ++j) {
+            const uint64_t who = __ballot(z[j] >= enters);
+            if (who) {
+              const int n = total - from + __popcll(who & ((1ull << lane) - 1));
+              const uint32_t i = at + tile.place(j);
+              if ((who >> lane & 1) && n >= 0 && n < 64)
+                cand[n] = ((uint64_t)ordered(z[j]) << 32) | (0xFFFFFFFFu - i);
+              total += __popcll(who);
+            }
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          const int n = min(64, total - from);
+          if (n > SC_FEW) {
+            top.merge_up(sort_up(lane < n ? cand[lane] : 0));
+          } else {
+            for (int c = 0; c < n; ++c) top.insert(cand[c], a.k);
+          }
+          asm volatile("" ::: "memory");
+        }
+        top.settle(a.k);
+        const uint32_t q = __builtin_amdgcn_readlane((uint32_t)(top.key >> 32), (a.k + 3) / 4 - 1);
+        if (lane == 0 && q) s_bar[wave] = unordered(q);
       }
     }
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
+  for (int o = 32; o > 0; o >>= 1)
     score_join(m, s, t, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), __shfl_xor(t, o, 64));
-    above += __shfl_xor(above, o, 64);
-  }
   if (lane == 0) {
     s_m[wave] = m;
     s_s[wave] = s;
     s_t[wave] = t;
     s_above[wave] = above;
   }
-  if (TOP) s_key[64 * wave + lane] = top.key;
+  // ascending, for the merge; what is behind the k-th key stays behind it
+  if (TOP) s_key[64 * wave + 63 - lane] = lane < a.k ? top.key : 0;
   __syncthreads();
   if (wave) return;
-  above = s_above[0];
   for (int w = 1; w < 4; ++w) {
     score_join(m, s, t, s_m[w], s_s[w], s_t[w]);
     above += s_above[w];
-    if (TOP)
-      for (int j = 0; j < a.k && top_offer(top, s_key[64 * w + j], a.k); ++j) {
-      }
+    if (TOP) top.merge_up(s_key[64 * w + lane]);
   }
   if (SPLIT) {
     const size_t o = (size_t)row * a.nseg + seg;
@@ -286,41 +397,37 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
 }
 
 // Joins a row's segments. The stats: one wave, a lane per segment. The lists:
-// all into LDS at once (the merge walks them with dependent steps, which would
-// each cost a memory round trip), then four waves merge a quarter of them each
-// and the first one the four results.
+// all into LDS at once (a merge waits for its list), then four waves merge a
+// quarter of them each and the first one the four results.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(SC_T) void k_score_join(ScoreArgs a) {
   __shared__ uint64_t s_key[TOP ? SC_MAX_SEG * DSV4G_MAX_TOP : 1];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
-  ScorePart p = {SC_LOW, 0.0f, 0.0f, 0};
+  ScorePart p = {-__builtin_inff(), 0.0f, 0.0f, 0};
   if (lane < a.nseg) p = a.part[(size_t)row * a.nseg + lane];
   const int token = a.tokens ? a.tokens[row] : -1;
   const bool have = token >= 0 && token < a.vocab;
+  float zt = 0.0f;
+  if (have) {
+    const T e = ((const T *)a.logits)[(size_t)row * a.stride + token];
+    zt = fmaf(sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16), a.scale, 0.0f);
+  }
   TopList top;
   top.init();
   if (TOP) {
     const uint64_t *keys = a.keys + (size_t)row * a.nseg * a.k;
     for (int i = tid; i < a.nseg * a.k; i += SC_T) s_key[i] = keys[i];
     __syncthreads();
-    for (int g = wave; g < a.nseg; g += 4)
-      for (int j = 0; j < a.k && top_offer(top, s_key[g * a.k + j], a.k); ++j) {
-      }
+    const int r = 63 - lane;  // ascending
+    for (int g = wave; g < a.nseg; g += 4) top.merge_up(r < a.k ? s_key[g * a.k + r] : 0);
     __syncthreads();
-    s_key[64 * wave + lane] = top.key;
+    s_key[64 * wave + r] = top.key;
     __syncthreads();
   }
   if (wave) return;
   if (TOP)
-    for (int w = 1; w < 4; ++w)
-      for (int j = 0; j < a.k && top_offer(top, s_key[64 * w + j], a.k); ++j) {
-      }
-  float zt = 0.0f;
-  if (have) {
-    const T e = ((const T *)a.logits)[(size_t)row * a.stride + token];
-    zt = fmaf(sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16), a.scale, 0.0f);
-  }
+    for (int w = 1; w < 4; ++w) top.merge_up(s_key[64 * w + lane]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     score_join(p.m, p.s, p.t, __shfl_xor(p.m, o, 64), __shfl_xor(p.s, o, 64),

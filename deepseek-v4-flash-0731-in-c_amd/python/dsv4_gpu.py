@@ -104,47 +104,58 @@ def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
-# ---- argument checks of the entries that take whole tensors
-def _same_device(who, *tensors):
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and (t.device != dev or not t.is_cuda):
-            raise ValueError(f"{who}: tensors must be on one GPU")
+# ---- argument checks of the entries that take whole tensors. They run on
+# every call of a decode loop, whose kernels take a few microseconds: device
+# numbers and data types are compared, nothing is built.
+def _same_device(who, first, *others):
+    """The GPU that all tensors are on."""
+    d = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != d:
+            d = -1
+    if d < 0:
+        raise ValueError(f"{who}: tensors must be on one GPU")
+    return d
 
 
 def _int32(who, t, n):
     import torch
-    if t is not None and (t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous()):
+    if t is not None and (t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous()):
         raise ValueError(f"{who}: contiguous int32 tensor of {n} entries needed, got "
                          f"{t.dtype} {tuple(t.shape)}")
 
 
-def _act_dtype(who, *tensors):
+def _act_dtype(who, first, other=None):
     """DSV4G_DT_F32 or _BF16 of float32 / bfloat16 tensors of one type."""
     import torch
-    kinds = {t.dtype for t in tensors if t is not None}
-    if kinds == {torch.float32}:
-        return DTYPE_CODES["F32"]
-    if kinds == {torch.bfloat16}:
-        return DTYPE_CODES["BF16"]
-    raise ValueError(f"{who}: float32 or bfloat16 tensors of one type needed, got {kinds}")
+    kind = first.dtype
+    if other is None or other.dtype is kind:
+        if kind is torch.float32:
+            return DTYPE_CODES["F32"]
+        if kind is torch.bfloat16:
+            return DTYPE_CODES["BF16"]
+    raise ValueError(f"{who}: float32 or bfloat16 tensors of one type needed, got {kind}"
+                     + (f" and {other.dtype}" if other is not None else ""))
 
 
 def _rows(who, t, heads, dim):
     """Elements from token to token of [tokens][heads][dim] with whole rows."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1 or \
-            (heads > 1 and t.stride(1) != dim):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or stride[2] != 1 or \
+            (heads > 1 and stride[1] != dim):
         raise ValueError(f"{who}: [tokens][{heads}][{dim}] with contiguous rows needed, got "
-                         f"{tuple(t.shape)} with strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else heads * dim
+                         f"{tuple(shape)} with strides {stride}")
+    return stride[0] if shape[0] > 1 else heads * dim
 
 
-def _workspace(workspace, need, device):
-    """The caller's workspace if it is large enough, else a fresh one."""
+def _at(t):
+    """A tensor's address for an entry's void * (None: NULL)."""
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(need, device):
     import torch
-    if workspace is None or workspace.nbytes < need:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
-    return workspace
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
 
 
 class GpuLib:
@@ -276,6 +287,18 @@ class GpuLib:
         self._call("dsv4g_argmax", _ptr(idx), _ptr(logits), vocab, n, vocab, self._stream())
         return idx
 
+    def _on(self, device, name, *args):
+        """Entry `name` on a device number's current stream."""
+        import torch
+        fn = getattr(self.lib, name)
+        if torch._C._cuda_getDevice() == device:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        else:
+            with torch.cuda.device(device):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        if rc != 0:
+            raise RuntimeError(f"{name}: {self.lib.dsv4g_last_error().decode()}")
+
     def logprobs_workspace_bytes(self, vocab, n, top=0):
         return int(self.lib.dsv4g_logprobs_workspace_bytes(vocab, n, top))
 
@@ -290,65 +313,59 @@ class GpuLib:
             raise ValueError("logprobs: logits must be [n][vocab] with contiguous rows")
         n, vocab = logits.shape
         dt = _act_dtype("logprobs", logits)
-        _same_device("logprobs", logits, tokens, workspace)
+        d = _same_device("logprobs", logits, tokens, workspace)
         _int32("logprobs", tokens, n)
-        with torch.cuda.device(logits.device):
-            need = self.logprobs_workspace_bytes(vocab, n, top)
-            workspace = _workspace(workspace, need, logits.device)
-            f = dict(dtype=torch.float32, device=logits.device)
-            i = dict(dtype=torch.int32, device=logits.device)
-            logprob = rank = ids = top_lp = None
-            entropy = torch.empty(n, **f)
-            if tokens is not None:
-                logprob, rank = torch.empty(n, **f), torch.empty(n, **i)
-            if top:
-                ids, top_lp = torch.empty(n, top, **i), torch.empty(n, top, **f)
-            self._call("dsv4g_logprobs", _ptr(logprob), _ptr(entropy), _ptr(rank), _ptr(ids),
-                       _ptr(top_lp), _ptr(logits), dt, vocab, n, max(logits.stride(0), vocab),
-                       _ptr(tokens), top, scale, _ptr(workspace), workspace.nbytes,
-                       self._stream())
+        if not 0 <= top <= MAX_TOP:
+            raise ValueError(f"logprobs: top {top}, 0 to {MAX_TOP} needed")
+        if workspace is None:
+            workspace = _workspace(self.logprobs_workspace_bytes(vocab, n, top), logits.device)
+        f = dict(dtype=torch.float32, device=logits.device)
+        i = dict(dtype=torch.int32, device=logits.device)
+        logprob = rank = ids = top_lp = None
+        entropy = torch.empty(n, **f)
+        if tokens is not None:
+            logprob, rank = torch.empty(n, **f), torch.empty(n, **i)
+        if top:
+            ids, top_lp = torch.empty((n, top), **i), torch.empty((n, top), **f)
+        self._on(d, "dsv4g_logprobs", _at(logprob), entropy.data_ptr(), _at(rank), _at(ids),
+                 _at(top_lp), logits.data_ptr(), dt, vocab, n, max(logits.stride(0), vocab),
+                 _at(tokens), top, scale, workspace.data_ptr(), workspace.nbytes)
         return logprob, entropy, rank, ids, top_lp
 
     # ---- paged cache and the attention over it
     def cache_workspace_bytes(self, cache):
-        return int(self.lib.dsv4g_cache_workspace_bytes(C.byref(cache.struct)))
+        return int(self.lib.dsv4g_cache_workspace_bytes(cache.arg))
 
     def cache_init(self, cache):
         """Every sequence empty, every page free."""
-        import torch
-        with torch.cuda.device(cache.device):
-            self._call("dsv4g_cache_init", C.byref(cache.struct), self._stream())
+        self._on(cache.index, "dsv4g_cache_init", cache.arg)
 
     def cache_status(self, cache):
         """The cache's sticky status word (0: fine; CACHE_FULL, CACHE_LIST,
-        CACHE_PAGE), cleared."""
-        import torch
+        CACHE_PAGE), cleared; synchronises."""
         st = C.c_uint(0)
-        with torch.cuda.device(cache.device):
-            self._call("dsv4g_cache_status", C.byref(st), C.byref(cache.struct), self._stream())
+        self._on(cache.index, "dsv4g_cache_status", C.byref(st), cache.arg)
         return st.value
 
     def cache_reserve(self, cache, starts, seqs=None, workspace=None):
         """dsv4g_cache_reserve: room for starts[i + 1] - starts[i] new tokens
         of each listed sequence (int32 tensors)."""
-        import torch
         n = starts.numel() - 1
-        _same_device("cache_reserve", cache.pages, starts, seqs, workspace)
+        d = _same_device("cache_reserve", cache.pages, starts, seqs, workspace)
         _int32("cache_reserve", starts, n + 1)
         _int32("cache_reserve", seqs, n)
-        with torch.cuda.device(cache.device):
-            workspace = _workspace(workspace, self.cache_workspace_bytes(cache), cache.device)
-            self._call("dsv4g_cache_reserve", C.byref(cache.struct), _ptr(seqs), _ptr(starts), n,
-                       _ptr(workspace), workspace.nbytes, self._stream())
+        if workspace is None:
+            workspace = _workspace(self.cache_workspace_bytes(cache), cache.device)
+        self._on(d, "dsv4g_cache_reserve", cache.arg, _at(seqs), starts.data_ptr(), n,
+                 workspace.data_ptr(), workspace.nbytes)
 
     def cache_append(self, cache, layer, k, v, starts, seqs=None):
         """dsv4g_cache_append: k [tokens][kv_heads][k_dim] and v likewise (None
         where the values are the keys) into one layer's pages; tokens may be
         strided."""
-        import torch
         s = cache.struct
         n = starts.numel() - 1
-        _same_device("cache_append", cache.pages, k, v, starts, seqs)
+        d = _same_device("cache_append", cache.pages, k, v, starts, seqs)
         _int32("cache_append", starts, n + 1)
         _int32("cache_append", seqs, n)
         dt = _act_dtype("cache_append", k, v)
@@ -356,47 +373,39 @@ class GpuLib:
         vs = 0 if v is None else _rows("cache_append", v, s.kv_heads, s.v_dim)
         if v is not None and v.shape[0] != k.shape[0]:
             raise ValueError("cache_append: k and v of different lengths")
-        with torch.cuda.device(cache.device):
-            self._call("dsv4g_cache_append", C.byref(s), layer, _ptr(k), ks, _ptr(v), vs, dt,
-                       _ptr(seqs), _ptr(starts), n, k.shape[0], self._stream())
+        self._on(d, "dsv4g_cache_append", cache.arg, layer, k.data_ptr(), ks, _at(v), vs, dt,
+                 _at(seqs), starts.data_ptr(), n, k.shape[0])
 
     def cache_fork(self, cache, parents, children):
         """dsv4g_cache_fork: empty sequence children[i] shares parents[i]'s pages."""
-        import torch
         n = children.numel()
-        _same_device("cache_fork", cache.pages, parents, children)
+        d = _same_device("cache_fork", cache.pages, parents, children)
         _int32("cache_fork", parents, n)
         _int32("cache_fork", children, n)
-        with torch.cuda.device(cache.device):
-            self._call("dsv4g_cache_fork", C.byref(cache.struct), _ptr(parents), _ptr(children),
-                       n, self._stream())
+        self._on(d, "dsv4g_cache_fork", cache.arg, parents.data_ptr(), children.data_ptr(), n)
 
     def cache_free(self, cache, seqs, new_len=None):
         """dsv4g_cache_free: the listed sequences cut back to new_len tokens
         (None: 0)."""
-        import torch
         n = seqs.numel()
-        _same_device("cache_free", cache.pages, seqs, new_len)
+        d = _same_device("cache_free", cache.pages, seqs, new_len)
         _int32("cache_free", seqs, n)
         _int32("cache_free", new_len, n)
-        with torch.cuda.device(cache.device):
-            self._call("dsv4g_cache_free", C.byref(cache.struct), _ptr(seqs), _ptr(new_len), n,
-                       self._stream())
+        self._on(d, "dsv4g_cache_free", cache.arg, seqs.data_ptr(), _at(new_len), n)
 
     def cache_compact(self, cache, n_used=None, workspace=None):
         """dsv4g_cache_compact; n_used (int32 [1], optional) takes the number
         of pages in use."""
-        import torch
-        _same_device("cache_compact", cache.pages, n_used, workspace)
+        d = _same_device("cache_compact", cache.pages, n_used, workspace)
         _int32("cache_compact", n_used, 1)
-        with torch.cuda.device(cache.device):
-            workspace = _workspace(workspace, self.cache_workspace_bytes(cache), cache.device)
-            self._call("dsv4g_cache_compact", C.byref(cache.struct), _ptr(n_used),
-                       _ptr(workspace), workspace.nbytes, self._stream())
+        if workspace is None:
+            workspace = _workspace(self.cache_workspace_bytes(cache), cache.device)
+        self._on(d, "dsv4g_cache_compact", cache.arg, _at(n_used), workspace.data_ptr(),
+                 workspace.nbytes)
 
     def attention_workspace_bytes(self, cache, heads, n_seqs, n_tokens, max_q, max_kv):
-        return int(self.lib.dsv4g_attention_workspace_bytes(
-            C.byref(cache.struct), heads, n_seqs, n_tokens, max_q, max_kv))
+        return int(self.lib.dsv4g_attention_workspace_bytes(cache.arg, heads, n_seqs, n_tokens,
+                                                            max_q, max_kv))
 
     def attention(self, cache, layer, q, starts, seqs=None, max_q=None, max_kv=None, scale=None,
                   window=0, sink=None, out=None, lse=None, with_lse=False, workspace=None):
@@ -408,33 +417,35 @@ class GpuLib:
         s = cache.struct
         n, tokens = starts.numel() - 1, q.shape[0]
         heads = q.shape[1] if q.dim() == 3 else 0
-        _same_device("attention", cache.pages, q, starts, seqs, sink, out, lse, workspace)
+        d = _same_device("attention", cache.pages, q, starts, seqs, sink, out, lse, workspace)
         _int32("attention", starts, n + 1)
         _int32("attention", seqs, n)
         qs = _rows("attention", q, heads, s.k_dim)
         dv = s.v_dim or s.k_dim
         max_q = tokens if max_q is None else max_q
         max_kv = s.max_pages * s.page_size if max_kv is None else max_kv
-        with torch.cuda.device(cache.device):
-            if out is None:
-                out = torch.empty(tokens, heads, dv, dtype=q.dtype, device=q.device)
-            if lse is None and with_lse:
-                lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
-            dt = _act_dtype("attention", q, out)
+        if out is None:
+            out = torch.empty((tokens, heads, dv), dtype=q.dtype, device=q.device)
+            os_ = heads * dv
+        else:
             os_ = _rows("attention", out, heads, dv)
-            for t, size in ((lse, tokens * heads), (sink, heads)):
-                if t is not None and (t.dtype != torch.float32 or t.numel() != size or
-                                      not t.is_contiguous()):
-                    raise ValueError("attention: lse and sink must be contiguous float32, "
-                                     "[tokens][heads] and [heads]")
             if out.shape[0] != tokens:
                 raise ValueError("attention: out and q of different lengths")
-            workspace = _workspace(workspace, self.attention_workspace_bytes(
+        if lse is None and with_lse:
+            lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+        for t, size in ((lse, tokens * heads), (sink, heads)):
+            if t is not None and (t.dtype is not torch.float32 or t.numel() != size or
+                                  not t.is_contiguous()):
+                raise ValueError("attention: lse and sink must be contiguous float32, "
+                                 "[tokens][heads] and [heads]")
+        if workspace is None:
+            workspace = _workspace(self.attention_workspace_bytes(
                 cache, heads, n, tokens, max_q, max_kv), q.device)
-            self._call("dsv4g_attention", _ptr(out), os_, _ptr(lse), _ptr(q), qs, dt, C.byref(s),
-                       layer, heads, _ptr(seqs), _ptr(starts), n, tokens, max_q, max_kv,
-                       s.k_dim ** -0.5 if scale is None else scale, window, _ptr(sink),
-                       _ptr(workspace), workspace.nbytes, self._stream())
+        self._on(d, "dsv4g_attention", out.data_ptr(), os_, _at(lse), q.data_ptr(), qs,
+                 _act_dtype("attention", q, out), cache.arg, layer, heads, _at(seqs),
+                 starts.data_ptr(), n, tokens, max_q, max_kv,
+                 s.k_dim ** -0.5 if scale is None else scale, window, _at(sink),
+                 workspace.data_ptr(), workspace.nbytes)
         return out if lse is None else (out, lse)
 
     def expert_workspace_bytes(self, inter):
@@ -723,6 +734,7 @@ class DeviceLayer:
 
 
 CACHE_FULL, CACHE_LIST, CACHE_PAGE = 1, 2, 4  # DSV4G_CACHE_*: bits of the status word
+MAX_TOP = 64  # DSV4G_MAX_TOP
 
 
 class PagedCache:
@@ -748,7 +760,9 @@ class PagedCache:
         _int32("PagedCache", status, 1)
         self.pages, self.ref, self.table, self.length = pages, ref, table, length
         self.status, self.device = status, pages.device
+        self.index = pages.get_device()
         s = self.struct = DSV4GCache()
+        self.arg = C.byref(s)
         for name, t in (("pages", pages), ("ref", ref), ("table", table), ("len", length),
                         ("status", status)):
             setattr(s, name, t.data_ptr())
