@@ -100,6 +100,7 @@ struct Cfg {
   static constexpr int NO = at_max(1, NP / KW);  // tiles that a wave ends up with, if any
   static constexpr int PART = (KW - 1) * NO * 4096, JOIN = KW > 1 ? 4 * PART + 2048 : 0;
   static constexpr int LDS = at_max(NTILE * STAGE + NRAW * RAW, JOIN);
+  static_assert(!OK || RW < 4 || LDS >= ROWS * 2 * D, "the result's rows pass through LDS");
   // The next stage's loads go between the products (issued at once they hold up
   // the wave): of a full tile, bound by the products, between all of them;
   // with fewer rows, bound by the memory, between those of the first half.
@@ -168,7 +169,12 @@ __device__ __forceinline__ void one(Item &it) {
 // Shared work (fewer items than the chip has places for): the stages of all
 // items in a row, items ordered by (sequence, tile), then kv head, are dealt
 // out in equal runs, so that long and short sequences fill every workgroup
-// alike. Workgroup w takes stages [w T / W, (w + 1) T / W).
+// alike. Workgroup w takes stages [w T / W, (w + 1) T / W). Between two items
+// lie AT_START stages with no work: what it costs a workgroup to end one item
+// and begin another, so that those which do have fewer stages (64 sequences of
+// 130 to 8100 E4M3 tokens: 90 us with 0, 68, 63 and 64 with 3, 6 and 10; with
+// equal lengths up to 3% lost).
+constexpr int AT_START = 6;
 __device__ __forceinline__ int shared_groups(const AttnArgs &a, long total) {
   return (int)(total < a.groups ? total : a.groups);
 }
@@ -197,7 +203,7 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
   long mine = 0;
   Item it;
   for (int j = j0; j < j1; ++j)
-    if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, it)) mine += it.stages;
+    if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, it)) mine += it.stages + AT_START;
   long x = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -213,7 +219,7 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
     total += s_sum[w];
   }
   before *= C.kv_heads;
-  p.total = one(total * C.kv_heads);
+  p.total = one(total * C.kv_heads - (total ? AT_START : 0));  // none behind the last item
   const int groups = shared_groups(a, p.total);
   p.at = p.end = 0;
   if ((int)blockIdx.x >= groups) return;
@@ -222,11 +228,12 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
   if (p.at >= before && p.at < before + mine * C.kv_heads)
     for (int j = j0; j < j1; ++j)
       if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, it)) {
-        const long all = (long)it.stages * C.kv_heads;
+        const int span = it.stages + AT_START;
+        const long all = (long)span * C.kv_heads;
         if (p.at < before + all) {
           s_at[0] = j;
-          s_at[1] = (int)((p.at - before) / it.stages);
-          s_at[2] = (int)((p.at - before) % it.stages);
+          s_at[1] = (int)((p.at - before) / span);
+          s_at[2] = (int)((p.at - before) % span);
           s_item = it;
           break;
         }
@@ -258,6 +265,14 @@ __device__ __forceinline__ void lds_load4(uint32_t to, uint32_t at, I4 rsrc) {
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// What the waves wrote to LDS is there for all of them. Not __syncthreads():
+// that waits for the loads of later stages, too.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // Brings stages of an item to LDS, PER loads per wave: begin() looks at the
@@ -505,6 +520,56 @@ __device__ __forceinline__ void store_tile(const AttnArgs &a, size_t row_at, int
   }
 }
 
+// The same for a whole tile of 32 rows (n of them live, lane % 32's at
+// `row_at`), through LDS: a lane holds 8 bytes of its row at a time, which would
+// be partial writes of 32 rows per store; so the wave writes its rows to its
+// part of LDS, chunks swizzled as in the stages, and reads them back along the
+// rows, whole lines per store.
+template <int D>
+__device__ __forceinline__ void store_rows(const AttnArgs &a, size_t row_at, int n, uint32_t lds,
+                                           int lane, const F16v *o, float f) {
+  lds_barrier();  // every wave is done with the stages
+  fresh(lane);
+  const uint32_t to = lds + lane % 32 * (2 * D) + 16 * chunk_swizzle<D>(lane % 32) +
+                      8 * (lane / 32);
+  each<D / 32>([&](auto d) {
+    const F16v y = tile_out(o[d]);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t c = dim_of<D>(d, g / 2) / 8 + g % 2;
+      DSV4_LDS(U2, to ^ (16 * c)) = U2{pack_bf16(y[4 * g] * f, y[4 * g + 1] * f),
+                                             pack_bf16(y[4 * g + 2] * f, y[4 * g + 3] * f)};
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  });
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  constexpr int CH = D / 8, RI = 64 / CH;  // chunks of a row, rows per store
+  constexpr int U = at_min(8, 32 / RI);    // stores at a time
+  for (int i = 0; i < 32; i += RI * U) {
+    U4 x[U];
+    size_t at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = i + u * RI + lane / CH;
+      x[u] = DSV4_LDS(U4, lds + r * (2 * D) + 16 * (lane % CH ^ chunk_swizzle<D>(r)));
+      at[u] = __shfl(row_at, r, 64) + lane % CH * 8;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u * RI + lane / CH >= n) continue;
+      if (a.f32) {
+        float4 *p = (float4 *)((float *)a.out + at[u]);
+        p[0] = make_float4(u2f(x[u][0] << 16), u2f(x[u][0] & 0xFFFF0000u), u2f(x[u][1] << 16),
+                           u2f(x[u][1] & 0xFFFF0000u));
+        p[1] = make_float4(u2f(x[u][2] << 16), u2f(x[u][2] & 0xFFFF0000u), u2f(x[u][3] << 16),
+                           u2f(x[u][3] & 0xFFFF0000u));
+      } else {
+        *(U4 *)((uint16_t *)a.out + at[u]) = x[u];
+      }
+    }
+  }
+}
+
 // The denominator's reciprocal (0 where nothing was seen) and lse, with the
 // head's sink joined. m in units of log2.
 __device__ __forceinline__ float finish_row(const AttnArgs &a, int head, float m, float l,
@@ -568,13 +633,22 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     it.kvh = w.kvh;
     one(it);
     const int s0 = w.stage;
+    if (s0 >= it.stages) {  // between this item and the next
+      w.at += it.stages + AT_START - s0;
+      w.stage = 0;
+      if (++w.kvh == C.kv_heads) {
+        w.kvh = 0;
+        ++w.pair;
+      }
+      continue;
+    }
     const int s1 = one(a.groups ? (int)min((long)it.stages, s0 + w.end - w.at) : it.stages);
     if (a.groups) {
       if (s0 == 0 && tid == 0) {
         a.first[1 + (long)w.pair * C.kv_heads + it.kvh] = w.at;
         if (w.at == 0) a.first[0] = w.total;
       }
-      w.at += s1 - s0;
+      w.at += s1 - s0 + AT_START;
       w.stage = 0;
       if (++w.kvh == C.kv_heads) {
         w.kvh = 0;
@@ -621,7 +695,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       }
     }
     // not 0: a hidden score stays -inf when it is scaled
-    const float c2 = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);
+    const float c2 = fmaxf(fabsf(a.scale) * LOG2E, 1.4e-45f);
 
     F16v o[NP];
 #pragma unroll
@@ -651,14 +725,10 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       // before st
       constexpr int AHEAD = F::TWICE ? 1 : 0;
       wait_loads<(RING - 2 - AHEAD) * F::PER>();
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
+      lds_barrier();
       if (FP8 && !F::TWICE) {
         convert<D, SHARED, TT>(raw0 + i % RING * RSTEP, lds0, tid);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+        lds_barrier();
       }
       const int next = st + RING - 1;
       load.begin(C, G, a, it, next, next < s1, ring0 + (i + RING - 1) % RING * RSTEP, wave);
@@ -670,20 +740,19 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       // sees it is not finite then: by its score, or as below)
       uint32_t odd = 0;
       if (min(w0 + TT, it.hi) - 1 > shown || (a.window && max(w0, it.clear) <= hidden)) {
-        constexpr int PT = 256 / TT, NB = 2 * D / PT;  // threads per token, bytes of each
+        constexpr int PT = 256 / TT, NC = D / 8 / PT;  // threads per token, chunks of each
         const int t = tid / PT;
-        const uint32_t at = lds0 + here + (SHARED ? 0 : F::KB) + t * (2 * D) +
-                            tid % PT * NB;
+        const uint32_t at = lds0 + here + (SHARED ? 0 : F::KB) + t * (2 * D) + tid % PT * 16;
         uint32_t big = 0;
 #pragma unroll
-        for (int j = 0; j < NB / 16; ++j) {
-          const U4 x = DSV4_LDS(U4, at + 16 * j);
+        for (int j = 0; j < NC; ++j) {
+          const U4 x = DSV4_LDS(U4, at + 16 * PT * j);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             big |= ((x[k] & 0x7F80u) == 0x7F80u) | ((x[k] & 0x7F800000u) == 0x7F800000u);
         }
         if (big) atomicOr(&s_odd[t / 32], 1u << (t % 32));
-        __syncthreads();
+        lds_barrier();
         uint32_t any = 0;
 #pragma unroll
         for (int k = 0; k < F::KW; ++k) any |= s_odd[k];
@@ -731,15 +800,17 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         if (__any(mt > m + AT_GROW)) {
           const float M = fmaxf(m, mt);
           const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
+          if (i) {  // else O is 0
+#pragma unroll
+            for (int d = 0; d < NP; ++d) {
+              F16v y = tile_out(o[d]);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) y[i] *= f;
+              tile_in(o[d], y);
+            }
+          }
           m = M;
           l *= f;
-#pragma unroll
-          for (int d = 0; d < NP; ++d) {
-            F16v y = tile_out(o[d]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] *= f;
-            tile_in(o[d], y);
-          }
         }
         const float mu = m > -__builtin_inff() ? m : 0.0f;
         U4 b0, b1;
@@ -759,7 +830,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       if (F::TWICE && st + 1 < s1)
         convert<D, SHARED, TT>(raw0 + (i + 1) % RING * RSTEP, lds0 + (i + 1) % 2 * STAGE, tid);
       if (odd) {
-        __syncthreads();  // every wave has its scores
+        lds_barrier();  // every wave has its scores
         const int t = tid % TT;
         if (s_odd[t / 32] >> (t % 32) & 1) {
           const uint32_t at = lds0 + here + (SHARED ? 0 : F::KB) + t * (2 * D);
@@ -770,7 +841,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
           const int t = t0 + __builtin_ctz(left);
           if (t <= pos && (!a.window || t > pos - a.window)) l = __builtin_nanf("");
         }
-        __syncthreads();
+        lds_barrier();
         if (tid < F::KW) s_odd[tid] = 0;  // read again two barriers on at the earliest
       }
       {
@@ -850,6 +921,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         }
       });
     }
+    float rinv = 0.0f;
     if (active && wr0 + lane % 32 < it.nrows) {
       if (s0 > 0 || s1 < it.stages) {
         const size_t slot = 2 * (size_t)blockIdx.x + (s0 == 0);  // the run's last item, or its first
@@ -869,13 +941,21 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         float lse;
         const float r = finish_row(a, head, m, l, &lse);
         const size_t row = (size_t)(it.start + tok);
-        each<NP>([&](auto d) {
-          if (KW == 1 || d / NO == kw)
-            store_tile<D>(a, row * a.out_stride + (size_t)head * D, d, h, tile_out(o[d]), r);
-          __builtin_amdgcn_sched_barrier(0);
-        });
+        if constexpr (KW == 1)
+          rinv = r;
+        else
+          each<NP>([&](auto d) {
+            if (d / NO == kw)
+              store_tile<D>(a, row * a.out_stride + (size_t)head * D, d, h, tile_out(o[d]), r);
+            __builtin_amdgcn_sched_barrier(0);
+          });
         if (a.lse && kw == 0 && h == 0) a.lse[row * a.heads + head] = lse;
       }
+    }
+    if constexpr (KW == 1) {
+      if (s0 == 0 && s1 == it.stages)
+        store_rows<D>(a, (size_t)(it.start + tok) * a.out_stride + (size_t)head * D,
+                      it.nrows - wr0, lds0 + wave * (32 * 2 * D), lane, o, rinv);
     }
     if (!a.groups) return;
     __syncthreads();  // the stages' LDS is free again
@@ -1015,8 +1095,11 @@ static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_toke
   const int places = D == 64    ? attn_places<64, false>(p.rw, fp8)
                      : D == 128 ? attn_places<128, false>(p.rw, fp8)
                                 : 256;
-  // two items per place and more: each whole; fewer: their stages dealt out
-  p.groups = p.items < 2 * places ? places : 0;
+  // Three items per place and more: each whole. Fewer: their stages dealt out.
+  // 512 items on 256 places (64 sequences, 8 kv heads of 128): 76 us dealt out
+  // and 87 whole at lengths of 100 to 4000, 198 and 189 where all have 4000;
+  // 800 short ones (10 to 1000 tokens of 512): 141 and 115.
+  p.groups = p.items < 3 * places ? places : 0;
   p.bytes = 0;
   if (p.groups)
     p.bytes = (size_t)p.groups * 2 * 32 * p.rw * (D * sizeof(float) + sizeof(float2)) +
