@@ -797,20 +797,19 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         mx = fmaxf(mx, z[15]);
         mx = swap_max(mx);
         const float mt = mx * c2;
+        m = i ? m : mt;  // nothing to rescale yet
         if (__any(mt > m + AT_GROW)) {
           const float M = fmaxf(m, mt);
           const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
-          if (i) {  // else O is 0
-#pragma unroll
-            for (int d = 0; d < NP; ++d) {
-              F16v y = tile_out(o[d]);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] *= f;
-              tile_in(o[d], y);
-            }
-          }
           m = M;
           l *= f;
+#pragma unroll
+          for (int d = 0; d < NP; ++d) {
+            F16v y = tile_out(o[d]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] *= f;
+            tile_in(o[d], y);
+          }
         }
         const float mu = m > -__builtin_inff() ? m : 0.0f;
         U4 b0, b1;
