@@ -14,7 +14,7 @@
 //  - K tiles are read row by row (16 bytes), V tiles by the transposing LDS
 //    read, both from the same row-major tile: where the values are the keys,
 //    a cached row is staged once for both products.
-// Weights are rounded to BF16 for the matrix unit (2^-9 relative, as the cache
+// Weights are rounded to BF16 for the matrix unit (2^-8 relative, as the cache
 // rows are BF16 themselves); scores, m, l and O stay in fp32. m follows the
 // maximum only when it grows by more than 2^8 (weights up to 2^8 lose nothing
 // in fp32 or BF16): the rescaling of O, one multiplication per accumulator, is
@@ -1162,7 +1162,10 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
     return dsv4g_fail(DSV4G_EINVAL, "attention: rows of q and out must be 16-byte aligned and at "
                       "least heads * dim apart");
   const AttnPlan p = attn_plan(C, heads, n_seqs, n_tokens, max_q);
-  if (p.items > 0x7FFFFFFFL || (long)max_q * (heads / C->kv_heads) > 0x7FFFFF00L)
+  // a launch is below 2^32 threads, a sequence's rows (new tokens * heads of a
+  // kv head) below 2^31
+  if (p.items > 0xFFFFFFL ||
+      (long)(max_q < n_tokens ? max_q : n_tokens) * (heads / C->kv_heads) > 0x7FFFFF00L)
     return dsv4g_fail(DSV4G_EINVAL, "attention: too many rows for one call");
   if (p.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.bytes))
     return dsv4g_fail(DSV4G_EINVAL, "attention: 256-byte aligned workspace of %zu bytes needed "
@@ -1171,7 +1174,10 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
   a.out = out, a.lse = lse, a.q = q, a.out_stride = out_stride, a.q_stride = q_stride;
   a.seqs = seqs, a.starts = starts, a.sink = sink, a.layer = layer, a.heads = heads;
   a.group = heads / C->kv_heads, a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.max_q = max_q;
-  a.max_kv = max_kv, a.window = window, a.f32 = act_dtype == DSV4G_DT_F32;
+  a.max_kv = max_kv, a.f32 = act_dtype == DSV4G_DT_F32;
+  // a window that no length passes is none: positions less the window then fit
+  // 32 bits
+  a.window = window < (long)C->max_pages * C->page_size ? window : 0;
   a.tiles = p.tiles, a.groups = p.groups, a.scale = scale;
   if (p.groups) {
     const size_t cells = (size_t)p.groups * 2 * 32 * p.rw;

@@ -10,8 +10,8 @@
 //   s' = f s1 + ..,    t' = f (t1 + (M1 - M') s1) + ..
 // and at the end, with d = m L - M, the rounding of M, exactly by an fma,
 //   lse - m = ln s - d ln 2,  entropy = ln s - (t / s) ln 2.
-// All in fp32, whose sums run over at most a few hundred terms per thread
-// before they are joined pairwise. A maximum below SC_LOW counts as SC_LOW (a
+// All in fp32, whose sums run over 1/256 of a row per thread (505 terms of
+// 129280) before they are joined pairwise. A maximum below SC_LOW counts as SC_LOW (a
 // row of nothing but a mask of the type's lowest value is even); -inf, a token
 // that cannot be taken, weighs nothing.
 //
@@ -486,6 +486,8 @@ int dsv4g_logprobs(float *logprob, float *entropy, int *rank, int *top_id, float
     return dsv4g_fail(DSV4G_EINVAL, "logprobs: logprob and rank need tokens");
   if ((uintptr_t)logits & (dtype == DSV4G_DT_F32 ? 3 : 1))
     return dsv4g_fail(DSV4G_EINVAL, "logprobs: misaligned logits");
+  if (vocab > 1 << 30 || n > 0xFFFFFF)  // places in 32 bits; a launch is below 2^32 threads
+    return dsv4g_fail(DSV4G_EINVAL, "logprobs: %d rows of %d, at most 2^24 - 1 of 2^30", n, vocab);
   const size_t need = dsv4g_logprobs_workspace_bytes(vocab, n, k);
   if (need && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need))
     return dsv4g_fail(DSV4G_EINVAL, "logprobs: 256-byte aligned workspace of %zu bytes needed "

@@ -149,7 +149,8 @@ int dsv4g_argmax(int *idx, const float *logits, int vocab, int n, size_t stride,
  * nothing. A token outside [0, vocab) gives a NaN logprob and rank -1; k above
  * vocab leaves id -1 and NaN behind the vocab entries. A row whose largest
  * logit is infinite, or that holds a NaN, has NaN log probabilities and
- * entropy and rank -1 (among the top k a NaN logit counts as -inf). workspace: 256-byte aligned, at least
+ * entropy and rank -1 (among the top k a NaN logit counts as -inf). n is below
+ * 2^24, vocab at most 2^30. workspace: 256-byte aligned, at least
  * dsv4g_logprobs_workspace_bytes(vocab, n, k) (0: none is needed, and it may
  * be NULL); a call uses nothing that an earlier one left there. No
  * counterpart in the reference. */
@@ -378,7 +379,8 @@ int dsv4g_ffn_step(float *state, const float *hc_fn, const float *hc_scale,
  * DSV4G_DT_BF16: two bytes each. DSV4G_DT_F8_E4M3: one code each, then in the
  * same order an E8M0 code per DSV4G_CACHE_GROUP columns
  * ([kv_heads][page_size][k_dim / 64], the values' after them); a value is
- * code * 2^(scale - 127). A page takes dsv4g_cache_page_bytes(C), a multiple
+ * code * 2^(scale - 127) (a scale code of 255 counts as 254; append writes
+ * 105 .. 247). A page takes dsv4g_cache_page_bytes(C), a multiple
  * of 256; page p of layer l is at pages + (l * n_pages + p) * that.
  *
  * Sequence s (a row of the table) holds len[s] tokens; its j-th token lies in
@@ -476,7 +478,7 @@ int dsv4g_cache_compact(const DSV4GCache *C, int *n_used, void *workspace,
  * lse: F32 [n_tokens][heads], optional. The outputs of a call that sets a
  * status bit are not valid. max_q, max_kv: host bounds of the
  * listed counts and lengths (a sequence beyond them is skipped with a status
- * bit); they size the launch. seqs may name a sequence more than once.
+ * bit); they size the launch, so close ones are faster. seqs may name a sequence more than once.
  * workspace: 256-byte aligned, at least dsv4g_attention_workspace_bytes (0:
  * none is needed, and it may be NULL); a call uses nothing that an earlier
  * one left there. */

@@ -190,6 +190,39 @@ def test_hidden_tokens_have_no_influence(env, shape, fp8, new):
         assert (~torch.isfinite(out[bad_new:].float())).any(-1).all()
 
 
+@pytest.mark.parametrize("shape,fp8", [(LATENT, False), (GQA, True)], ids=str)
+def test_window_that_no_length_passes(env, shape, fp8):
+    """The largest windows are no window, in tiles whose first rows see
+    nothing of the last stages."""
+    s = Setup(env, shape, 32, fp8, [60, 0], [90, 33], seed=8)
+    out, lse = s.run()
+    s.check(out, lse, rows={0, 1, 40, 89, 90, 122})
+    for window in (2**31 - 1, 2**31 - 200, 65536, 150):
+        again, again_lse = s.run(window=window)
+        assert env["torch"].equal(out, again) and env["torch"].equal(lse, again_lse), window
+
+
+@pytest.mark.parametrize("shape", [LATENT, GQA], ids=str)
+def test_scale_of_zero(env, shape):
+    """Every visible token weighs the same, however large the products are."""
+    torch = env["torch"]
+    s = Setup(env, shape, 16, False, [70, 3], [5, 1], seed=9)
+    s.q *= 1e16
+    starts, total = [0, 75], [75, 4]
+    for value in (1.0, 1e16):
+        env["lib"].cache_append(s.c, 1, s.k * value, s.v, ints(env, [0, 75, 79]))
+        out, lse = s.run(scale=0.0)
+        rows = (s.k * value if s.v is None else s.v).to(torch.bfloat16).double()
+        for r, (b, p) in enumerate([(0, 70), (0, 71), (0, 72), (0, 73), (0, 74), (1, 3)]):
+            seen = rows[starts[b]:starts[b] + p + 1]
+            want = seen.mean(0).repeat_interleave(shape[0] // shape[1], 0)
+            mass = seen.abs().mean(0).repeat_interleave(shape[0] // shape[1], 0)
+            # weights exactly 1, sums in fp32; the result rounded once
+            tol = 2.0 ** -8 * want.abs() + (p + 8) * 2.0 ** -24 * mass
+            assert ((out[r].double() - want).abs() <= tol).all(), (value, r)
+            assert ((lse[r].double() - math.log(p + 1)).abs() <= 1e-6).all()
+
+
 def test_values_not_finite_in_seen_places(env):
     """Separate values with an infinity in one column: rows that see it are not
     finite there, rows that do not see it are as without."""

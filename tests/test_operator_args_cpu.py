@@ -100,6 +100,21 @@ def test_append_refusals(raw, bad):
                                   a["dt"], a["seqs"], a["starts"], a["n"], a["tokens"], None) == 1
 
 
+def test_launches_too_large(raw):
+    c = C.byref(cache())
+    assert raw.dsv4g_cache_append(c, 0, P, 256, P, 256, F32, P, P, 2, 1 << 26, None) == 1
+    assert b"2^26" in raw.dsv4g_last_error()
+    for n, vocab in ((1 << 24, 8), (1, (1 << 30) + 1)):
+        assert raw.dsv4g_logprobs(P, P, P, P, P, P, F32, vocab, n, vocab, P, 1, 1.0, P, 1 << 40,
+                                  None) == 1
+        assert b"2^24" in raw.dsv4g_last_error()
+    # 2^24 items: as many (sequence, kv head) pairs
+    a = GOOD_ATT
+    assert raw.dsv4g_attention(P, a["os"], P, P, a["qs"], BF16, c, 1, 8, P, P, 1 << 23, 1 << 23,
+                               1, 100, 0.1, 0, P, P, 1 << 40, None) == 1
+    assert b"too many rows" in raw.dsv4g_last_error()
+
+
 def test_append_values_of_a_latent_cache(raw):
     c = cache(k_dim=512, v_dim=0, kv_heads=1)
     a = GOOD_APPEND
