@@ -27,14 +27,15 @@
 // at least k of the tile's values reach it. Two sorted lists merge in 6 steps:
 // the larger of a[i] and b[63 - i] is the upper half of both, a bitonic sequence.
 //
-// Bound: HBM for fp32 rows (2048 rows of 129280: 196 us, 5.4 TB/s), the vector
-// units for BF16 ones, with half the bytes per value (156 us, 3.4 TB/s: 8.5
-// instructions a value, one of them 2^x at a quarter of the rate). k = 8 adds 18
-// and 58 us: a wave looks through its first tiles and then ever fewer. Fewer
-// registers for it (six waves per SIMD in place of five) cost 10%: the sort's
-// lane masks are then computed at each use.
+// Bound: HBM for fp32 rows (2048 rows of 129280: 179 us, 5.9 TB/s), the vector
+// units for BF16 ones, with half the bytes per value (125 us, 4.2 TB/s: about 10
+// instructions a value, one of them 2^x at a quarter of the rate; with the
+// index compared for every value's rank it was 156). k = 8 adds 15 and 59 us: a
+// wave looks through its first tiles and then ever fewer. Fewer registers for
+// it (six waves per SIMD in place of five) cost 10%: the sort's lane masks are
+// then computed at each use.
 // Rows are cut into segments until a launch has about 2048 workgroups, what the
-// chip holds at once; a second launch joins them (64 rows 13 us, one row 17 us,
+// chip holds at once; a second launch joins them (64 rows 12 us, one row 17 us,
 // against 278 and 303 us in library calls).
 #include "dsv4_device.h"
 #include "dsv4_gpu_internal.h"
@@ -275,6 +276,8 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
     const T e = l[token];
     zt = fmaf(sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16), a.scale, 0.0f);
   }
+  // the next value below it (no z is -0)
+  const float zt_below = unordered(ordered(zt) - (zt == 0.0f ? 2 : 1));
   if (TOP) {
     if (tid < 4) s_bar[tid] = -__builtin_inff();
     __syncthreads();
@@ -309,11 +312,18 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
       for (int j = 0; j < SC_E; ++j)
         s += z[j] > -__builtin_inff() ? 1.0f : z[j] == z[j] ? 0.0f : z[j];
     }
-    // rank: equal values count where they come first (few tiles reach the token's)
+    // rank: equal values count where they come first; but for the token's own
+    // tile, one comparison does it
     if (__any(mt >= zt)) {
+      if (zt > -__builtin_inff() && (at + SC_TILE <= token || at > token)) {
+        const float th = at < token ? zt_below : zt;
 #pragma unroll
-      for (int j = 0; j < SC_E; ++j)
-        above += __popcll(__ballot(z[j] > zt || (z[j] == zt && at + tile.place(j) < token)));
+        for (int j = 0; j < SC_E; ++j) above += __popcll(__ballot(z[j] > th));
+      } else {
+#pragma unroll
+        for (int j = 0; j < SC_E; ++j)
+          above += __popcll(__ballot(z[j] > zt || (z[j] == zt && at + tile.place(j) < token)));
+      }
     }
     if constexpr (TOP) {
       // Four waves' (k / 4)-th values or better are k values of the row: nothing

@@ -73,6 +73,28 @@ def test_orders_and_ties(env, n):
         check(env, z, [13] * n, 64, 1.0, rows=[0])
 
 
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+def test_equal_values_around_the_token(env, kind):
+    """Ranks of tokens whose value also stands in the tiles before and behind
+    theirs: zeros of both signs, the values next to them, infinities, the
+    type's lowest value; whole rows per workgroup and rows in segments."""
+    torch, dev = env["torch"], env["dev"]
+    t = getattr(torch, kind)
+    info = torch.finfo(t)
+    tiny = torch.nextafter(torch.zeros((), dtype=t), torch.ones((), dtype=t)).item()
+    some = torch.tensor([0.0, -0.0, tiny, -tiny, 1.0, -1.0, info.min, float("-inf")], dtype=t,
+                        device=dev)
+    v = 3 * 4096 + 5
+    g = torch.Generator(device=dev).manual_seed(12)
+    for n in (2050, 3):
+        z = some[torch.randint(0, 8, (n, v), generator=g, device=dev)]
+        tokens = [(4096 * (r % 4) + [0, 4, 4095, -1][r // 4 % 4]) % v for r in range(n)]
+        # every value in turn at the token's place
+        z[torch.arange(n, device=dev), torch.tensor(tokens, device=dev)] = \
+            some[torch.arange(n, device=dev) % 8]
+        check(env, z, tokens, 3, 1.0, rows=[r for r in range(0, 64) if r < n])
+
+
 def test_banned_and_bad_values(env):
     torch, dev = env["torch"], env["dev"]
     inf, nan = float("inf"), float("nan")
