@@ -23,6 +23,23 @@
 // Rows of 16-byte chunks are stored with the chunk index XORed by a function
 // of the row (chunk_swizzle): both kinds of read then touch every bank once
 // per 16 lanes.
+//
+// What bounds it, with 64 latent heads of 512 if nothing else is said:
+//  - a chunk of 2048 tokens behind 14336, BF16: the matrix unit beside LDS
+//    (every wave reads the whole tile: 128 KB per 32 tokens and product pair at
+//    128 bytes a clock against 2048 clocks of products). 3.95 ms, 1.04 PFLOP/s,
+//    79% of a large library product; E4M3 4.7 ms (the conversion).
+//  - decode over long caches: HBM. 64 sequences of 8100: BF16 130 us (4.1 TB/s),
+//    E4M3 131 us (the conversion again: half the bytes, the same LDS traffic);
+//    8 sequences of 16000 over 8 kv heads of 128, BF16: 103 us, 5.1 TB/s.
+//  - short ones: dependent latencies. One sequence of 1777: 18 us, of which
+//    finding the place 2.6, the item and its pages 2, the query rows 2.7, the
+//    first rows of the cache 1.4, the stages 2.2, the waves' exchange 3.1, the
+//    parts' stores 1.3; the launch that joins them 5.5.
+// Taken back: query rows asked for before the second stage's loads (a chunk 2%
+// faster, decode 1 to 3% slower), query rows first of all (spills).
+#include <algorithm>
+#include <cmath>
 #include <utility>
 
 #include "dsv4_cache.h"
@@ -96,7 +113,7 @@ struct Cfg {
   static constexpr int PER = FP8 ? M * (at_max(1, CODES / 4096) + at_max(1, TT / 64))
                                  : STAGE / 4096;
   // what the other waves of its rows hand a wave at the end: their parts of
-  // its tiles; then every wave's (m, l)
+  // its tiles; then every wave's (m, l). 0 with one wave per row.
   static constexpr int NO = at_max(1, NP / KW);  // tiles that a wave ends up with, if any
   static constexpr int PART = (KW - 1) * NO * 4096, JOIN = KW > 1 ? 4 * PART + 2048 : 0;
   static constexpr int LDS = at_max(NTILE * STAGE + NRAW * RAW, JOIN);
@@ -485,7 +502,9 @@ __device__ __forceinline__ Bf8 read_vt(uint32_t at, int u, int dt) {
   return __builtin_bit_cast(Bf8, r);
 }
 
-constexpr int AT_AHEAD = 6;  // LDS reads ahead of their product (even)
+// LDS reads ahead of their product: a read's latency is about four products,
+// and each one ahead takes four registers.
+constexpr int AT_AHEAD = 6;
 
 // An output tile moved between the accumulation registers, where it stays in
 // the loop, and the vector registers that arithmetic needs: one tile at a
@@ -524,7 +543,9 @@ __device__ __forceinline__ void store_tile(const AttnArgs &a, size_t row_at, int
 // `row_at`), through LDS: a lane holds 8 bytes of its row at a time, which would
 // be partial writes of 32 rows per store; so the wave writes its rows to its
 // part of LDS, chunks swizzled as in the stages, and reads them back along the
-// rows, whole lines per store.
+// rows, whole lines per store (128 rows of 512: 7.5 -> 5.3 us with every
+// workgroup storing at once, 6 TB/s). Tiles of fewer rows are stored as they are:
+// most of theirs are parts, which need no such thing.
 template <int D>
 __device__ __forceinline__ void store_rows(const AttnArgs &a, size_t row_at, int n, uint32_t lds,
                                            int lane, const F16v *o, float f) {
@@ -863,7 +884,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     l = swap_sum(l);
 
     // The waves that shared the rows: a wave hands the others their share of
-    // its output tiles through LDS and takes theirs of its own, NP / KW tiles.
+    // its output tiles through LDS and takes theirs of its own, NO tiles.
     constexpr int KW = F::KW, NO = F::NO;
     float f = 1.0f;                          // its own outputs' factor
     if constexpr (KW > 1) {
@@ -962,7 +983,10 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
 }
 
 // Joins the parts of every item that several workgroups shared: a workgroup
-// per output tile of a row wave, whose four waves take every fourth part.
+// per output tile of a row wave, whose four waves take every fourth part (one
+// wave for all of them took 107 us for the 251 parts of one sequence of 16000;
+// that whole call now takes 46). Bound by latency (5.5 us for 28 parts), then by the parts' bytes
+// (11 us for the 33 MB of 64 latent sequences).
 template <int D, int RW>
 __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   constexpr int TT = 32 * (4 / RW), ROWS = 32 * RW, NP = D / 32;
@@ -1079,10 +1103,14 @@ static int attn_places(int rw, bool fp8) {  // workgroups that the chip holds
                 : rw == 2 ? (fp8 ? Cfg<D, SHARED, true, 2>::WGS : Cfg<D, SHARED, false, 2>::WGS)
                           : (fp8 ? Cfg<D, SHARED, true, 4>::WGS : Cfg<D, SHARED, false, 4>::WGS));
 }
-static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_tokens, int max_q) {
+// A window's plan takes no workspace where that of none takes none: the longest
+// item only gets shorter.
+static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_tokens, int max_q,
+                          int max_kv, int window) {
   AttnPlan p;
   max_q = max_q > n_tokens ? n_tokens : max_q;
-  const long rows = (long)max_q * (heads / C->kv_heads);
+  const int group = heads / C->kv_heads;
+  const long rows = (long)max_q * group;
   const int D = C->k_dim;
   // the smallest tile that holds a sequence's rows
   const int least = D == 512 || (D == 256 && C->v_dim) ? 2 : 1;
@@ -1094,11 +1122,23 @@ static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_toke
   const int places = D == 64    ? attn_places<64, false>(p.rw, fp8)
                      : D == 128 ? attn_places<128, false>(p.rw, fp8)
                                 : 256;
-  // Three items per place and more: each whole. Fewer: their stages dealt out.
-  // 512 items on 256 places (64 sequences, 8 kv heads of 128): 76 us dealt out
-  // and 87 whole at lengths of 100 to 4000, 198 and 189 where all have 4000;
-  // 800 short ones (10 to 1000 tokens of 512): 141 and 115.
-  p.groups = p.items < 3 * places ? places : 0;
+  // Three items per place and more: each whole. Fewer: their stages are dealt
+  // out where that saves more than it costs, in stages of the longest item that
+  // the host's bounds allow (S). Whole items leave the chip idle for the rest of
+  // their last round, or half a longest item where lengths differ; dealt out,
+  // they pay a second start, the join's launch (3) and the parts, written and
+  // read: 16 per workgroup where a part is 64 rows of 512.
+  // 64 sequences of up to 4000, 8 kv heads of 128 (512 items, 256 places): 76 us
+  // dealt out, 87 whole; 198 and 189 where all have 4000. 800 sequences of up to
+  // 1000, latent 512: 141 and 115. 11 prompts of 82 tokens, latent 512 (451 items
+  // of 3 stages): 96 and 43.
+  const long kv = std::min<long>(max_kv, (long)C->max_pages * C->page_size);
+  const int TT = 32 * (4 / p.rw);
+  const long span = window ? std::min<long>(kv, (long)window + 32 * p.rw / group + 31) : kv;
+  const double S = (double)((span + TT - 1) / TT), r = (double)p.items / places;
+  const double idle = std::max(std::ceil(r) - r, 0.5) * (S + AT_START);
+  const double parts = p.rw * D / 64.0 * std::min(1.0, p.items * S / (2.0 * places));
+  p.groups = r < 3 && idle > AT_START + 3 + parts ? places : 0;
   p.bytes = 0;
   if (p.groups)
     p.bytes = (size_t)p.groups * 2 * 32 * p.rw * (D * sizeof(float) + sizeof(float2)) +
@@ -1140,7 +1180,7 @@ size_t dsv4g_attention_workspace_bytes(const DSV4GCache *C, int heads, int n_seq
   if (!C || !cache_geom(C, &G) || heads <= 0 || heads % C->kv_heads || n_seqs <= 0 ||
       n_tokens <= 0 || max_q <= 0 || max_kv <= 0)
     return 0;
-  return attn_plan(C, heads, n_seqs, n_tokens, max_q).bytes;
+  return attn_plan(C, heads, n_seqs, n_tokens, max_q, max_kv, 0).bytes;
 }
 
 int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, size_t q_stride,
@@ -1161,7 +1201,10 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
       q_stride % unit || out_stride % unit || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))
     return dsv4g_fail(DSV4G_EINVAL, "attention: rows of q and out must be 16-byte aligned and at "
                       "least heads * dim apart");
-  const AttnPlan p = attn_plan(C, heads, n_seqs, n_tokens, max_q);
+  // a window that no length passes is none: positions less the window then fit
+  // 32 bits
+  if (window >= (long)C->max_pages * C->page_size) window = 0;
+  const AttnPlan p = attn_plan(C, heads, n_seqs, n_tokens, max_q, max_kv, window);
   // a launch is below 2^32 threads, a sequence's rows (new tokens * heads of a
   // kv head) below 2^31
   if (p.items > 0xFFFFFFL ||
@@ -1174,10 +1217,7 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
   a.out = out, a.lse = lse, a.q = q, a.out_stride = out_stride, a.q_stride = q_stride;
   a.seqs = seqs, a.starts = starts, a.sink = sink, a.layer = layer, a.heads = heads;
   a.group = heads / C->kv_heads, a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.max_q = max_q;
-  a.max_kv = max_kv, a.f32 = act_dtype == DSV4G_DT_F32;
-  // a window that no length passes is none: positions less the window then fit
-  // 32 bits
-  a.window = window < (long)C->max_pages * C->page_size ? window : 0;
+  a.max_kv = max_kv, a.window = window, a.f32 = act_dtype == DSV4G_DT_F32;
   a.tiles = p.tiles, a.groups = p.groups, a.scale = scale;
   if (p.groups) {
     const size_t cells = (size_t)p.groups * 2 * 32 * p.rw;

@@ -69,7 +69,9 @@ __global__ void k_cache_clear_status(unsigned *status) { *status = 0; }
 // Room for the new tokens of n listed sequences: a thread per sequence counts
 // the pages it needs, the pool is scanned from its start until enough free
 // pages are found, and only then anything is changed. One workgroup; bound by
-// the latency of its dependent steps (list -> length -> table -> ref -> scan).
+// the latency of its dependent steps (list -> length -> table -> ref -> scan):
+// 9.4 us for 16 sequences and 512 pages, and no less with the counts loaded
+// ahead.
 __global__ __launch_bounds__(CB_T) void k_cache_reserve(DSV4GCache C, const int *seqs,
                                                         const int *starts, int n, int *ws) {
   __shared__ int s_seq[CB_T], s_page[CB_T], s_off[CB_T], s_at[CB_T], s_copy[CB_T];
@@ -175,7 +177,10 @@ __global__ __launch_bounds__(CB_T) void k_cache_reserve(DSV4GCache C, const int 
 // Moves the pages of the workspace's list, every layer's (items of 16 KB, 4
 // 16-byte loads in flight per thread), and with remap the table entries of the
 // pages that moved. The list's pages are all different and no destination is
-// a source, so nothing is ordered. Bound by HBM.
+// a source, so nothing is ordered. Bound by HBM: 536 MB in 107 us (5.0 TB/s; a
+// pool of 2048 pages and 16 layers). 46 MB over 43 layers' pages take 20 us,
+// 2.3 TB/s: first touches of pages all over a pool of 0.7 GB. Items of even size
+// and 32-bit divisions changed neither.
 constexpr int CM_CHUNK = 16384;
 __global__ __launch_bounds__(256) void k_cache_move(DSV4GCache C, int *ws, size_t page_bytes,
                                                     int remap) {
@@ -325,8 +330,9 @@ __global__ __launch_bounds__(CB_T) void k_cache_compact(DSV4GCache C, int *n_use
 // ------------------------------------------------------------------ append
 // One wave per new token: its place by counting the starts at or before its
 // row, then 8 columns per lane and step (8 neighbouring lanes are one scale
-// group of 64 columns). Bound: HBM for many tokens, the latency of starts ->
-// sequence -> length -> table entry -> store for few.
+// group of 64 columns). Bound: HBM for many tokens (4096 of 8 kv heads of 128
+// and 128: 53 MB in 11.3 us, 4.7 TB/s), the latency of starts -> sequence ->
+// length -> table entry -> store for few (64 latent rows: 4.2 us).
 template <bool F32, bool FP8>
 __global__ __launch_bounds__(256) void k_cache_append(DSV4GCache C, CacheGeom G, int layer,
                                                       const void *k, size_t k_stride,

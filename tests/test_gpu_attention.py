@@ -190,6 +190,33 @@ def test_hidden_tokens_have_no_influence(env, shape, fp8, new):
         assert (~torch.isfinite(out[bad_new:].float())).any(-1).all()
 
 
+@pytest.mark.parametrize("shape", [LATENT, SHARD, LAT256, GQA, ONE, ODD, WIDE, MHA], ids=str)
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("window", [0, 45])
+def test_items_whole_and_dealt_out(env, shape, fp8, window):
+    """The same batches under a close bound of their lengths (whole items) and
+    under a wide one, which has their stages dealt out over the chip: decode,
+    drafts and a chunk, with sequences that have nothing new between them."""
+    gpu, lib = env["gpu"], env["lib"]
+    for past, new in (([70, 0, 3, 200, 129], [1, 1, 1, 1, 0]), ([100, 31, 0], [5, 0, 5]),
+                      ([40, 7], [150, 61])):
+        s = Setup(env, shape, 16, fp8, past, new, seed=len(past))
+        n, heads, kvh, kd, vd = len(past), *shape
+        table = env["torch"].full((n, 4096), -1, dtype=env["torch"].int32, device=env["dev"])
+        table[:, :s.c.table.shape[1]] = s.c.table
+        c = gpu.PagedCache(s.c.pages, s.c.ref, table, s.c.length, s.c.status, 16, kvh, kd, vd,
+                           "fp8" if fp8 else "bf16")
+        most = [max(p + m for p, m in zip(past, new)), 65536]
+        rows = set(range(0, sum(new), 13)) | {sum(new) - 1}
+        need = [lib.attention_workspace_bytes(c, heads, n, sum(new), max(new), kv) for kv in most]
+        assert need[1] > 0
+        for kv in most:
+            out, lse = lib.attention(c, 1, s.q, s.starts, max_q=max(new), max_kv=kv,
+                                     window=window, with_lse=True)
+            s.check(out, lse, window, rows=rows)
+        assert lib.cache_status(c) == 0
+
+
 @pytest.mark.parametrize("shape,fp8", [(LATENT, False), (GQA, True)], ids=str)
 def test_window_that_no_length_passes(env, shape, fp8):
     """The largest windows are no window, in tiles whose first rows see
