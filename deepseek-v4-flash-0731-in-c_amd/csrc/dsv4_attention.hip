@@ -25,10 +25,11 @@
 // per 16 lanes.
 //
 // What bounds it, with 64 latent heads of 512 if nothing else is said:
-//  - a chunk of 2048 tokens behind 14336, BF16: the matrix unit beside LDS
-//    (every wave reads the whole tile: 128 KB per 32 tokens and product pair at
-//    128 bytes a clock against 2048 clocks of products). 3.95 ms, 1.04 PFLOP/s,
-//    79% of a large library product; E4M3 4.7 ms (the conversion).
+//  - a chunk of 2048 tokens behind 14336, BF16: LDS reads beside the matrix unit.
+//    Of the 4700 clocks that 32 tokens take, the products are 2048 (the unit is
+//    busy 42% of the time) and the reads, each wave the whole tile, as many at
+//    128 bytes a clock; the softmax between them 450. 3.95 ms, 1.04 PFLOP/s, 79%
+//    of a large library product; E4M3 4.7 ms (the conversion).
 //  - decode over long caches: HBM. 64 sequences of 8100: BF16 130 us (4.1 TB/s),
 //    E4M3 131 us (the conversion again: half the bytes, the same LDS traffic);
 //    8 sequences of 16000 over 8 kv heads of 128, BF16: 103 us, 5.1 TB/s.
