@@ -229,6 +229,7 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
     if (lane >= o) x += y;
   }
   if (lane == 63) s_sum[wave] = x;
+  if (tid == 0) s_at[0] = pairs;  // no place
   __syncthreads();
   long before = x - mine, total = 0;
 #pragma unroll
@@ -642,8 +643,9 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     w.end = 1;
   }
   if (bad) return;
-  // One segment after the other: a run of stages of one item.
-  for (bool first = true; w.at < w.end; first = false) {
+  // One segment after the other: a run of stages of one item. (The pairs end with
+  // the run, unless something else changes the lengths meanwhile.)
+  for (bool first = true; w.at < w.end && w.pair < a.n_seqs * a.tiles; first = false) {
     Item it;
     if (first && a.groups) {
       it = w.it;  // looked up already
@@ -1006,8 +1008,10 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   Item it;
   if (bad || !attn_item<ROWS, TT>(C, a, pair / a.tiles, pair % a.tiles, it)) return;
   const int groups = shared_groups(a, total);
-  const int w0 = share_of(total, groups, at), w1 = share_of(total, groups, at + it.stages - 1);
-  if (w0 == w1) return;
+  if (groups <= 0) return;
+  const int w0 = max(0, share_of(total, groups, at));
+  const int w1 = min(groups - 1, share_of(total, groups, at + it.stages - 1));
+  if (w0 >= w1) return;
   const int r = it.r0 + 32 * rw + lane % 32;
   const bool live = r < it.nrows;  // parts hold such rows only
   // the first workgroup's part is its run's last, the others' their first

@@ -293,6 +293,31 @@ def test_rows_behind_the_last_and_strides(env):
     assert torch.equal(f, want.float()) and torch.equal(fl, wl)
 
 
+@pytest.mark.parametrize("shape", [LATENT, SHARD, LAT256, GQA, ONE, ODD, WIDE, MHA], ids=str)
+@pytest.mark.parametrize("kv", [64, 65536])
+def test_chunks_in_wider_buffers(env, shape, kv):
+    """As above for chunks, whose last tiles are not full: columns beside the
+    heads and rows around the sequences stay as they were, in both types."""
+    torch, lib, dev = env["torch"], env["lib"], env["dev"]
+    heads, kvh, kd, vd = shape
+    s = Setup(env, shape, 16, False, [9, 0, 1], [37, 0, 53], seed=10)
+    dv, n = vd or kd, 90
+    want, wl = lib.attention(s.c, 1, s.q, s.starts, max_q=53, max_kv=kv, with_lse=True)
+    s.check(want, wl, rows={0, 1, 17, 36, 37, 60, 88, 89})
+    for t in (torch.bfloat16, torch.float32):
+        obuf = torch.full((n + 7, heads * dv + 8), 3.0, dtype=t, device=dev)
+        out = obuf[:, :heads * dv].unflatten(1, (heads, dv))
+        lse = torch.full((n + 7, heads), 3.0, device=dev)
+        q = torch.zeros(n + 7, heads * kd + 16, dtype=t, device=dev)
+        q = q[:, 16:].unflatten(1, (heads, kd))
+        q[5:5 + n] = s.q
+        lib.attention(s.c, 1, q, s.starts + 5, max_q=53, max_kv=kv, out=out, lse=lse)
+        assert torch.equal(out[5:5 + n], want.to(t)) and torch.equal(lse[5:5 + n], wl)
+        for x in (obuf, lse):
+            assert (x[:5] == 3).all() and (x[5 + n:] == 3).all()
+        assert (obuf[:, heads * dv:] == 3).all()
+
+
 def test_many_sequences_and_repeats(env):
     """More sequences than a wave has lanes, listed in another order, some
     twice."""
