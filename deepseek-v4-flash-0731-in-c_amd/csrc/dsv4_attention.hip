@@ -25,11 +25,10 @@
 // per 16 lanes.
 //
 // What bounds it, with 64 latent heads of 512 if nothing else is said:
-//  - a chunk of 2048 tokens behind 14336, BF16: LDS reads beside the matrix unit.
-//    Of the 4700 clocks that 32 tokens take, the products are 2048 (the unit is
-//    busy 42% of the time) and the reads, each wave the whole tile, as many at
-//    128 bytes a clock; the softmax between them 450. 3.95 ms, 1.04 PFLOP/s, 79%
-//    of a large library product; E4M3 4.7 ms (the conversion).
+//  - a chunk of 2048 tokens behind 14336, BF16: 3.8 to 3.95 ms, 1.04 to 1.09
+//    PFLOP/s, 79 to 83% of a large library product's rate; the matrix unit is
+//    busy 42% of the time. Without the loads in the loop it would take 3.1 ms;
+//    half of the LDS reads changed nothing. E4M3 4.6 ms (the conversion).
 //  - decode over long caches: HBM. 64 sequences of 8100: BF16 130 us (4.1 TB/s),
 //    E4M3 131 us (the conversion again: half the bytes, the same LDS traffic);
 //    8 sequences of 16000 over 8 kv heads of 128, BF16: 103 us, 5.1 TB/s.
@@ -314,8 +313,20 @@ struct Loader {
   static_assert(F::PER == M * (ROWS_PER + NS), "loads of a stage");
   int page[NG], spage[at_max(1, NS)];  // of the next stage
   I4 rsrc[NG], srsrc[at_max(1, NS)];   // of this one
-  int t0, w0;                          // its first token, the wave's of it
+  int t0;                              // its first token
   uint32_t lds;
+  // This lane's offset from a load's first row. A load's rows are a multiple of
+  // TB on, and the swizzle moves bits only, so that of row base + o is that of
+  // base XOR that of o: a load costs a few instructions for its address. (All of
+  // it computed per lane: a latent chunk 2% slower, 32 short sequences over 8 kv
+  // heads 12%.)
+  uint32_t lane_at;  // rows of less than a load, else it is 16 * lane
+
+  __device__ __forceinline__ void init(int lane) {
+    const int o = lane * TB / 64;
+    lane_at = o * (2 * D) + 16u * ((lane % (D / 8)) ^ chunk_swizzle<D>(o));
+    if constexpr (!FP8 && TB > 1) asm volatile("" : "+v"(lane_at));
+  }
 
   __device__ __forceinline__ int row_group(int wave, int g) const {
     return (wave * NG + g) * TG % TT;
@@ -366,25 +377,27 @@ struct Loader {
   template <int K>
   __device__ __forceinline__ void load(const DSV4GCache &C, const CacheGeom &G, const Item &it,
                                        int wave, int lane) const {
-    fresh(lane);
     constexpr int m = K % M, i = K / M;
     const int head = it.kvh * C.page_size, mask = C.page_size - 1;
     if constexpr (i < ROWS_PER) {
       constexpr int g = i / (TG / TB), j = i % (TG / TB);
-      const int tl0 = row_group(wave, g), off = j * TB + lane * TB / 64;
-      const int slot = head + ((t0 + tl0) & mask) + off, tok = t0 + tl0 + off;
-      const bool in = tok < it.hi && tok >= it.clear;
-      uint32_t v, to;
-      if (FP8) {
-        v = (uint32_t)slot * D + lane * 16 % D;
-        to = lds + (tl0 + j * TB) * D + m * (F::CODES + F::SCALES);
+      const int tl0 = row_group(wave, g);
+      const int slot = head + ((t0 + tl0) & mask) + j * TB, tok = t0 + tl0 + j * TB;
+      constexpr int ROW = FP8 ? D : 2 * D;  // bytes
+      const uint32_t to = lds + (tl0 + j * TB) * ROW + m * (FP8 ? F::CODES + F::SCALES : F::KB);
+      fresh(lane);
+      uint32_t v = FP8 || TB == 1 ? 16u * lane : lane_at;
+      if (!FP8) v ^= 16u * chunk_swizzle<D>(tl0 + j * TB);
+      const uint32_t base = (uint32_t)slot * ROW + (m ? G.v_off : 0);
+      if constexpr (TB == 1) {  // the whole load is one token
+        v += tok < it.hi && tok >= it.clear ? base : AT_OUT;
       } else {
-        constexpr int CH = D / 8;
-        v = (uint32_t)slot * (2 * D) + 16u * ((lane % CH) ^ chunk_swizzle<D>(tl0 + off));
-        to = lds + (tl0 + j * TB) * (2 * D) + m * F::KB;
+        const uint32_t o = lane * TB / 64;
+        v = o + (uint32_t)(tok - it.clear) < (uint32_t)(it.hi - it.clear) ? v + base : AT_OUT;
       }
-      lds_load16(to, in ? v + (m ? G.v_off : 0) : AT_OUT, rsrc[g]);
+      lds_load16(to, v, rsrc[g]);
     } else {
+      fresh(lane);
       constexpr int S = D / 64, LANES = 4 * S;  // codes of a token, lanes of a load
       const int tl0 = scale_group(wave, i - ROWS_PER);
       const int slot = head + ((t0 + tl0) & mask), tok = t0 + tl0 + 4 * lane / S;
@@ -504,9 +517,10 @@ __device__ __forceinline__ Bf8 read_vt(uint32_t at, int u, int dt) {
   return __builtin_bit_cast(Bf8, r);
 }
 
-// LDS reads ahead of their product: a read's latency is about four products,
-// and each one ahead takes four registers.
-constexpr int AT_AHEAD = 6;
+// LDS reads ahead of their product (even): a read's latency is about four
+// products; 6 measured the same within 1%, 8 has too few registers left (5%
+// slower at decode).
+constexpr int AT_AHEAD = 4;
 
 // An output tile moved between the accumulation registers, where it stays in
 // the loop, and the vector registers that arithmetic needs: one tile at a
@@ -691,6 +705,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     const int pmax = one(pos0 + min(wr0 + 31, it.nrows - 1) / a.group);
 
     Loader<D, SHARED, FP8, RW> load;
+    load.init(lane);
     load.look(C, G, it, s0, wave);
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i) {
