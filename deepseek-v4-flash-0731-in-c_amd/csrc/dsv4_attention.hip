@@ -27,10 +27,10 @@
 // What bounds it, with 64 latent heads of 512 if nothing else is said:
 //  - a chunk of 2048 tokens behind 14336, BF16: 3.8 to 3.95 ms, 1.04 to 1.09
 //    PFLOP/s, 79 to 83% of a large library product's rate; the matrix unit is
-//    busy 42% of the time. Without the loads in the loop it would take 3.1 ms;
+//    busy 45% of the time. Without the loads in the loop it would take 3.1 ms;
 //    half of the LDS reads changed nothing. E4M3 4.6 ms (the conversion).
 //  - decode over long caches: HBM. 64 sequences of 8100: BF16 130 us (4.1 TB/s),
-//    E4M3 131 us (the conversion again: half the bytes, the same LDS traffic);
+//    E4M3 127 to 145 us (the conversion: half the bytes, the same LDS traffic);
 //    8 sequences of 16000 over 8 kv heads of 128, BF16: 103 us, 5.1 TB/s.
 //  - short ones: dependent latencies. One sequence of 1777: 18 us, of which
 //    finding the place 2.6, the item and its pages 2, the query rows 2.7, the
