@@ -70,6 +70,19 @@ typedef uint32_t U2 __attribute__((ext_vector_type(2)));
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float AT_GROW = 8.0f;  // log2 of what the weights may grow to before a rescaling
 
+// A row's sums are kept against its m, the largest product q.k so far less what
+// it may have grown since: weights are 2^((z - m) c2). The difference comes
+// first: 2^(z c2 - fl(m c2)), one instruction less, would carry the rounding of
+// m c2, which no 2^x holds once scores pass 2^30.
+__device__ __forceinline__ float attn_c2(float scale) {
+  // not 0: a hidden score stays -inf
+  return fmaxf(fabsf(scale) * LOG2E, 1.4e-45f);
+}
+// The factor that takes sums against m1 to m; 0 where m has seen nothing.
+__device__ __forceinline__ float ref_factor(float m1, float m, float c2) {
+  return m > -__builtin_inff() ? __builtin_amdgcn_exp2f((m1 - m) * c2) : 0.0f;
+}
+
 struct AttnArgs {
   void *out;
   float *lse;
@@ -608,19 +621,24 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, size_t row_at, int
 }
 
 // The denominator's reciprocal (0 where nothing was seen) and lse, with the
-// head's sink joined. m in units of log2.
+// head's sink joined. The sink's distance to m's score is taken by one fma: both
+// may be large.
 __device__ __forceinline__ float finish_row(const AttnArgs &a, int head, float m, float l,
                                             float *lse) {
-  float f = 1.0f;
-  if (a.sink) {
-    const float z = a.sink[head] * LOG2E, M = fmaxf(m, z);
-    if (M > -__builtin_inff()) {
-      f = exp2f(m - M);  // 0 where nothing was seen
-      l = l * f + exp2f(z - M);
-      m = M;
+  const float s = fmaxf(fabsf(a.scale), 1.4e-45f);
+  float f = 1.0f, top = m * s;
+  const float sink = a.sink ? a.sink[head] : -__builtin_inff();
+  if (sink != -__builtin_inff()) {
+    const float d = fmaf(m, s, -sink) * LOG2E;  // -inf where nothing was seen
+    if (d > 0.0f) {
+      l += exp2f(-d);
+    } else {
+      f = exp2f(d);
+      l = l * f + 1.0f;
+      top = sink;
     }
   }
-  *lse = l != 0.0f ? (m + log2f(l)) * LN2 : -__builtin_inff();
+  *lse = l != 0.0f ? top + log2f(l) * LN2 : -__builtin_inff();
   return l != 0.0f ? f / l : 0.0f;
 }
 
@@ -733,8 +751,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         q[s] = __builtin_bit_cast(Bf8, u ^ sign);
       }
     }
-    // not 0: a hidden score stays -inf when it is scaled
-    const float c2 = fmaxf(fabsf(a.scale) * LOG2E, 1.4e-45f);
+    const float c2 = attn_c2(a.scale);
 
     F16v o[NP];
 #pragma unroll
@@ -835,11 +852,10 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, z[i]), z[i + 1]);
         mx = fmaxf(mx, z[15]);
         mx = swap_max(mx);
-        const float mt = mx * c2;
-        m = i ? m : mt;  // nothing to rescale yet
-        if (__any(mt > m + AT_GROW)) {
-          const float M = fmaxf(m, mt);
-          const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
+        m = i ? m : mx;  // nothing to rescale yet
+        if (__any((mx - m) * c2 > AT_GROW)) {
+          const float M = fmaxf(m, mx);
+          const float f = ref_factor(m, M, c2);
           m = M;
           l *= f;
 #pragma unroll
@@ -855,8 +871,8 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         float part[4] = {};
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const float x0 = __builtin_amdgcn_exp2f(fmaf(z[i], c2, -mu));
-          const float x1 = __builtin_amdgcn_exp2f(fmaf(z[i + 1], c2, -mu));
+          const float x0 = __builtin_amdgcn_exp2f((z[i] - mu) * c2);
+          const float x1 = __builtin_amdgcn_exp2f((z[i + 1] - mu) * c2);
           part[i / 2 % 4] += x0 + x1;
           if (i < 8) b0[i / 2] = pack_bf16(x0, x1);
           else b1[i / 2 - 4] = pack_bf16(x0, x1);
@@ -925,14 +941,13 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
       float M = m;
 #pragma unroll
       for (int k = 0; k < KW; ++k) M = fmaxf(M, xs[(k * RW + rw) * 64 + lane].x);
-      const float mu = M > -__builtin_inff() ? M : 0.0f;
-      f = __builtin_amdgcn_exp2f(m - mu);
+      f = ref_factor(m, M, c2);
       float fk[KW];
       l = 0.0f;
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         const float2 s = xs[(k * RW + rw) * 64 + lane];
-        fk[k] = __builtin_amdgcn_exp2f(s.x - mu);
+        fk[k] = ref_factor(s.x, M, c2);
         l += s.y * fk[k];
       }
       m = M;
@@ -1031,6 +1046,7 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   const bool live = r < it.nrows;  // parts hold such rows only
   // the first workgroup's part is its run's last, the others' their first
   auto slot = [&](int w) { return (2 * (size_t)w + (w == w0)) * ROWS + 32 * rw; };
+  const float c2 = attn_c2(a.scale);
   float m = -__builtin_inff(), l = 0.0f;
   F16v o;
 #pragma unroll
@@ -1054,15 +1070,14 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
     float M = m;
 #pragma unroll
     for (int k = 0; k < U; ++k) M = fmaxf(M, s[k].x);
-    const float mu = M > -__builtin_inff() ? M : 0.0f;
-    const float f = __builtin_amdgcn_exp2f(m - mu);
+    const float f = ref_factor(m, M, c2);
     m = M;
     l *= f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] *= f;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const float p = __builtin_amdgcn_exp2f(s[k].x - mu);
+      const float p = ref_factor(s[k].x, M, c2);
       l += s[k].y * p;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -1084,15 +1099,14 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   float M = m;
 #pragma unroll
   for (int k = 0; k < 3; ++k) M = fmaxf(M, s_l[k][lane].x);
-  const float mu = M > -__builtin_inff() ? M : 0.0f;
-  const float f0 = __builtin_amdgcn_exp2f(m - mu);
+  const float f0 = ref_factor(m, M, c2);
   l *= f0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] *= f0;
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     const float2 s = s_l[k][lane];
-    const float p = __builtin_amdgcn_exp2f(s.x - mu);
+    const float p = ref_factor(s.x, M, c2);
     l += s.y * p;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -1214,8 +1228,8 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
       layer >= C->n_layers || heads <= 0 || heads % C->kv_heads || max_q <= 0 || max_kv <= 0 ||
       window < 0 || (act_dtype != DSV4G_DT_F32 && act_dtype != DSV4G_DT_BF16))
     return dsv4g_fail(DSV4G_EINVAL, "attention: bad arguments");
-  if (!(fabsf(scale) <= 3.4028235e38f))
-    return dsv4g_fail(DSV4G_EINVAL, "attention: scale %g", scale);
+  if (!(fabsf(scale) * LOG2E <= 3.4028235e38f))  // scores are taken to base 2
+    return dsv4g_fail(DSV4G_EINVAL, "attention: scale %g, at most 2.35e38", scale);
   const size_t unit = act_dtype == DSV4G_DT_F32 ? 4 : 8;  // elements of 16 bytes
   if (q_stride < (size_t)heads * C->k_dim || out_stride < (size_t)heads * C->k_dim ||
       q_stride % unit || out_stride % unit || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))

@@ -467,7 +467,8 @@ int dsv4g_cache_compact(const DSV4GCache *C, int *n_used, void *workspace,
  * heads reads kv head h / (heads / kv_heads); the token at position p sees
  * positions max(0, p - window + 1) .. p (window 0: all up to p);
  *   out = sum_j e^(z_j) v_j / (sum_j e^(z_j) + e^(sink[h])), z_j = scale q.k_j,
- * lse = log of the denominator. sink: F32 [heads] or NULL (no such term).
+ * lse = log of the denominator. sink: F32 [heads] or NULL (no such term). q.k is
+ * summed in fp32 and must stay in its range; |scale| is at most 2.35e38.
  * Tokens that a row does not see have no influence on it, whatever they hold;
  * a row that sees a key or value that is not finite is not finite in the
  * columns concerned (which others are not is left open).

@@ -151,6 +151,23 @@ def attend64(q, keys, values, pos, scale, window, sink):
     return out, lse, mass, most
 
 
+def attend64_far(q, keys, values, pos, scale, sink):
+    """attend64 without a window for scores of any size: every term relative to
+    the largest one (beyond 2^53 the sum's logarithm is lost beside a score
+    even in 64 bits). (out, lse, sum of p |v|)."""
+    g = q.shape[0] // keys.shape[1]
+    k, v = (x[:pos + 1].permute(1, 0, 2).repeat_interleave(g, 0) for x in (keys, values))
+    z = scale * torch.matmul(k, q[:, :, None])[:, :, 0]
+    if sink is not None:
+        z = torch.cat([z, sink[:, None]], 1)
+    top = z.amax(1, keepdim=True)
+    p = torch.exp(z - top)
+    total = p.sum(1, keepdim=True)
+    p = (p / total)[:, None, :pos + 1]
+    return (torch.matmul(p, v)[:, 0], (top + total.log())[:, 0],
+            torch.matmul(p, v.abs())[:, 0])
+
+
 def attend_bounds(out, mass, most, dim):
     """How far a BF16 result may be from out, and lse from its own.
 

@@ -510,3 +510,79 @@ def test_speculative_step(env):
     assert lib.cache_status(c) == 0
     used = {e for r in (1, 2) for e in c.table[r].tolist() if e >= 0}
     assert {i for i, r in enumerate(c.ref.tolist()) if r} == used
+
+
+def wide_table(s, cols=4096):
+    """The cache of a Setup under a table wide enough for any bound of lengths."""
+    torch = s.env["torch"]
+    _, kvh, kd, vd = s.shape
+    table = torch.full((len(s.past), cols), -1, dtype=torch.int32, device=s.env["dev"])
+    table[:, :s.c.table.shape[1]] = s.c.table
+    return s.env["gpu"].PagedCache(s.c.pages, s.c.ref, table, s.c.length, s.c.status, s.ps, kvh,
+                                   kd, vd, "fp8" if s.fp8 else "bf16")
+
+
+@pytest.mark.parametrize("shape", [LATENT, LAT256, GQA, ONE, WIDE], ids=str)
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_scores_of_any_size(env, shape, fp8):
+    """Scores up to the end of fp32's range, single tokens and long ranges
+    among the rows, items whole and dealt out, with and without a sink. Every
+    query has one column that is not zero, a power of two, so that q.k is exact
+    in fp32. What is left are the scaling's roundings, relative to the distance
+    to the row's maximum: 2^-22 of it, and e^-d d 2^-22 < 2^-23 of a weight,
+    within the bound's 2^-18 for a score of no size (attend_bounds)."""
+    torch, lib, dev = env["torch"], env["lib"], env["dev"]
+    heads, kvh, kd, vd = shape
+    past, new = [0, 700, 40, 0], [1, 3, 0, 70]
+    s = Setup(env, shape, 16, fp8, past, new, seed=21)
+    c = wide_table(s)
+    tokens, n = sum(new), len(past)
+    starts = s.starts.tolist()
+    host = s.c.pages[1].cpu()
+    held = [paged.rows64(host, s.table[b], past[b] + new[b], 16, kvh, kd, vd, fp8)
+            for b in range(n)]
+    g = torch.Generator(device=dev).manual_seed(5)
+    at = torch.randint(0, kd, (tokens, heads, 1), generator=g, device=dev)
+    rows = [0, 1, 3, 4, 73]
+    for exponent, scale in ((3, 1.0), (20, 1.0), (25, -0.7), (28, 1.0), (30, 1.3), (33, 1.0),
+                            (33, -1.0), (40, 1.0), (77, 0.3), (100, -1.0), (124, 1.0),
+                            (124, 3.0), (-100, 1e38), (-100, -2e38), (10, 1e-30)):
+        s.q.zero_()
+        s.q.scatter_(2, at, 2.0 ** exponent)
+        q, given = s.q.double().cpu(), float(torch.tensor(scale, dtype=torch.float32))
+        # the sink of each head is its first row's one score
+        own = given * held[0][0][0].repeat_interleave(heads // kvh, 0).gather(
+            1, at[0].cpu())[:, 0] * 2.0 ** exponent
+        for sink in (None, own.float()):
+            want = {}
+            for r in rows:
+                b = max(i for i in range(n) if starts[i] <= r and new[i])
+                want[r] = paged.attend64_far(q[r], *held[b], past[b] + r - starts[b], given,
+                                             None if sink is None else sink.double())
+            for kv in (773, 65536):
+                out, lse = lib.attention(c, 1, s.q, s.starts, max_q=max(new), max_kv=kv,
+                                         scale=scale, with_lse=True,
+                                         sink=None if sink is None else sink.to(dev))
+                out, lse = out.double().cpu(), lse.double().cpu()
+                for r, (o, e, mass) in want.items():
+                    tol, tol_lse = paged.attend_bounds(o, mass, torch.zeros_like(e), kd)
+                    where = (exponent, scale, kv, r)
+                    assert ((out[r] - o).abs() <= tol).all(), where
+                    assert ((lse[r] - e).abs() <= tol_lse + 2.0 ** -22 * e.abs()).all(), where
+    assert lib.cache_status(c) == 0
+
+
+def test_single_tokens_with_large_scores(env):
+    """A row that sees one token is that token's value, and its lse the score,
+    whatever the score's size: random rows, their products summed in fp32."""
+    torch, lib = env["torch"], env["lib"]
+    s = Setup(env, LATENT, 16, False, [0] * 40, [1] * 40, seed=22)
+    keys = s.k.to(torch.bfloat16).double()[:40]  # [sequence][1][512]
+    for size in (1.0, 1e6, 1e9, 3e9, 1e11, 1e20, 1e30):
+        q = (s.q.double() * size).to(torch.bfloat16)
+        out, lse = lib.attention(s.c, 1, q, s.starts, with_lse=True, scale=1.0)
+        assert torch.equal(out.double(), keys.expand(40, 64, 512)), size
+        z = (q.double() * keys).sum(2)
+        # 512 exact products summed in fp32, scaled once more
+        tol = 520 * 2.0 ** -24 * (q.double() * keys).abs().sum(2) + 1e-6
+        assert ((lse.double() - z).abs() <= tol).all(), size

@@ -186,3 +186,15 @@ def test_wrapper_refusals():
                             16, 1, 64, 64)
     with pytest.raises(ValueError, match="not a cache shape"):
         dsv4_gpu.PagedCache.new(1, 4, 17, 1, 64, 64, 1, 2, device="cpu")
+
+
+def test_scales_beyond_fp32_in_base_2(raw):
+    """A scale whose product with log2 e is no fp32 number is refused; the
+    largest that is one passes this check (and fails the next, its workspace)."""
+    c, a = C.byref(cache(max_pages=4096)), GOOD_ATT
+    top = 3.4028234663852886e38 / 1.4426950408889634
+    for scale, why in ((top * 1.001, b"scale"), (-3.4e38, b"scale"), (top * 0.999, b"workspace"),
+                       (-top * 0.999, b"workspace")):
+        assert raw.dsv4g_attention(P, a["os"], P, P, a["qs"], BF16, c, 1, 8, P, P, 2, 5, 5, 8192,
+                                   scale, 0, P, P, 0, None) == 1
+        assert why in raw.dsv4g_last_error(), scale
