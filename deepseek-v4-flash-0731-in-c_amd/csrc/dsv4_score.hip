@@ -5,15 +5,19 @@
 // One pass over the logits. With z = scale * logit and L = log2 e, every thread
 // keeps the running maximum m of its z and, with M = fl(m L),
 //   s = sum 2^(z L - M),  t = sum 2^(z L - M) (z L - M)
-// (one fma and the hardware's 2^x per logit); two such triples join as
-//   m' = max(m1, m2),  f = 2^(M1 - M'),
-//   s' = f s1 + ..,    t' = f (t1 + (M1 - M') s1) + ..
-// and at the end, with d = m L - M, the rounding of M, exactly by an fma,
-//   lse - m = ln s - d ln 2,  entropy = ln s - (t / s) ln 2.
+// (one fma and the hardware's 2^x per logit). Where |M| is SC_NEAR or more (masks
+// of -10^9 and beyond, in a thread that has seen nothing else, or the largest of
+// logits), M's rounding would grow until no 2^x holds it: there the exponent is
+// (z - m) L, one instruction more (taken everywhere, it costs 4% of 2048 BF16
+// rows). With off(m) what the first kind of M is off m L, exactly by an fma, two
+// triples join as
+//   m' = max(m1, m2),  g = (m1 - m') L + off(m1) - off(m'),  f = 2^g,
+//   s' = f s1 + ..,    t' = f (t1 + g s1) + ..
+// and at the end
+//   lse - m = ln s + off(m) ln 2,  entropy = ln s - (t / s) ln 2.
 // All in fp32, whose sums run over 1/256 of a row per thread (505 terms of
-// 129280) before they are joined pairwise. A maximum below SC_LOW counts as SC_LOW (a
-// row of nothing but a mask of the type's lowest value is even); -inf, a token
-// that cannot be taken, weighs nothing.
+// 129280) before they are joined pairwise. -inf, a token that cannot be taken,
+// weighs nothing.
 //
 // The top k are kept per wave, one key per lane in descending order (k <= 64):
 // (value as an ordered whole number, ~index), so keys are unique and equal
@@ -46,7 +50,7 @@ constexpr int SC_T = 256;              // threads
 constexpr int SC_E = 16;               // logits per thread and tile
 constexpr int SC_TILE = SC_T * SC_E;   // logits per tile: segments are multiples
 constexpr int SC_MAX_SEG = 64;         // segments of a row (one lane each when joined)
-constexpr float SC_LOW = -0x1p126f;    // least z in the sums (times L it is exact)
+constexpr float SC_NEAR = 0x1p16f;     // largest M of the sums by one fma
 constexpr float SC_L = 1.4426950408889634f, SC_LN2 = 0.6931471805599453f;
 constexpr int SC_FEW = 6;              // values that are inserted one by one
 
@@ -78,17 +82,23 @@ __device__ __forceinline__ float unordered(uint32_t o) {
   return u2f((o >> 31) ? o ^ 0x80000000u : ~o);
 }
 
-__device__ __forceinline__ float score_ref(float m) { return fmaxf(m, SC_LOW) * SC_L; }
-// f of a sum referred to M1, now to M, and its t.
-__device__ __forceinline__ float score_shift(float M1, float M, float s, float &t) {
-  const float f = __builtin_amdgcn_exp2f(M1 - M);
-  t = f * (t + fmaxf(M1 - M, -300.0f) * s);  // f is 0 below: no 0 * inf
+// What z is taken relative to: m, or the least number where all are -inf.
+__device__ __forceinline__ float score_ref(float m) { return fmaxf(m, -3.4028235e38f); }
+__device__ __forceinline__ float score_off(float m) {
+  const float M = m * SC_L;
+  return fabsf(M) < SC_NEAR ? -fmaf(m, SC_L, -M) : 0.0f;
+}
+// s of a sum relative to m1, now to m, and its t.
+__device__ __forceinline__ float score_shift(float m1, float m, float s, float &t) {
+  const float g = (m1 - m) * SC_L + (score_off(m1) - score_off(m));
+  const float f = __builtin_amdgcn_exp2f(g);
+  t = f * (t + fmaxf(g, -300.0f) * s);  // f is 0 below: no 0 * inf
   return f * s;
 }
 __device__ __forceinline__ void score_join(float &m, float &s, float &t, float m2, float s2,
                                            float t2) {
-  const float mm = fmaxf(m, m2), M = score_ref(mm);
-  s = score_shift(score_ref(m), M, s, t) + score_shift(score_ref(m2), M, s2, t2);
+  const float mm = fmaxf(m, m2), r = score_ref(mm);
+  s = score_shift(score_ref(m), r, s, t) + score_shift(score_ref(m2), r, s2, t2);
   t += t2;
   m = mm;
 }
@@ -235,15 +245,14 @@ __device__ __forceinline__ void score_write(const ScoreArgs &a, int row, float m
                                             float t, int above, uint64_t key, bool have_token,
                                             float zt) {
   // z - lse as (z - m) - (lse - m): m may be large
-  const float mc = fmaxf(m, SC_LOW);
-  const float ls = logf(s) - fmaf(mc, SC_L, -score_ref(m)) * SC_LN2;
+  const float ln = logf(s), ls = ln + score_off(score_ref(m)) * SC_LN2;
   const bool fine = s > 0.0f && m > -__builtin_inff();
   const int lane = threadIdx.x % 64;
   const float nan = __builtin_nanf("");
   if (lane == 0) {
     if (a.logprob) a.logprob[row] = have_token && fine ? (zt - m) - ls : nan;
     if (a.rank) a.rank[row] = have_token && fine ? above : -1;
-    if (a.entropy) a.entropy[row] = fine ? logf(s) - t / s * SC_LN2 : nan;
+    if (a.entropy) a.entropy[row] = fine ? ln - t / s * SC_LN2 : nan;
   }
   if (lane < a.k) {
     const size_t o = (size_t)row * a.k + lane;
@@ -282,7 +291,7 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
     if (tid < 4) s_bar[tid] = -__builtin_inff();
     __syncthreads();
   }
-  float m = -__builtin_inff(), M = score_ref(m), s = 0.0f, t = 0.0f;
+  float m = -__builtin_inff(), s = 0.0f, t = 0.0f;
   int above = 0;  // the wave's
   TopList top;
   top.init();
@@ -295,22 +304,25 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
 #pragma unroll
     for (int j = 2; j < SC_E; j += 2) mt = fmaxf(fmaxf(mt, z[j]), z[j + 1]);
     if (mt > m) {
+      s = score_shift(score_ref(m), score_ref(mt), s, t);
       m = mt;
-      const float N = score_ref(m);
-      s = score_shift(M, N, s, t);
-      M = N;
     }
-    if (m >= SC_LOW) {
+    const float M = m * SC_L;
+    if (fabsf(M) < SC_NEAR) {
 #pragma unroll
       for (int j = 0; j < SC_E; ++j) {
         const float d = fmaf(z[j], SC_L, -M), e = __builtin_amdgcn_exp2f(d);
         s += e;
-        t = fmaf(e, __builtin_amdgcn_fmed3f(d, -300.0f, 300.0f), t);  // no 0 * inf
+        t = fmaf(e, fmaxf(d, -300.0f), t);  // no 0 * inf
       }
-    } else {  // nothing above the least value yet: those there weigh 1, -inf nothing
+    } else {
+      const float r = score_ref(m);
 #pragma unroll
-      for (int j = 0; j < SC_E; ++j)
-        s += z[j] > -__builtin_inff() ? 1.0f : z[j] == z[j] ? 0.0f : z[j];
+      for (int j = 0; j < SC_E; ++j) {
+        const float d = (z[j] - r) * SC_L, e = __builtin_amdgcn_exp2f(d);
+        s += e;
+        t = fmaf(e, fmaxf(d, -300.0f), t);
+      }
     }
     // rank: equal values count where they come first; but for the token's own
     // tile, one comparison does it

@@ -147,9 +147,10 @@ int dsv4g_argmax(int *idx, const float *logits, int vocab, int n, size_t stride,
  *               lower index first where they are equal; their z - lse.
  * Outputs may be NULL. A logit of -inf is a token that cannot be taken: it adds
  * nothing. A token outside [0, vocab) gives a NaN logprob and rank -1; k above
- * vocab leaves id -1 and NaN behind the vocab entries. A row whose largest
- * logit is infinite, or that holds a NaN, has NaN log probabilities and
- * entropy and rank -1 (among the top k a NaN logit counts as -inf). n is below
+ * vocab leaves id -1 and NaN behind the vocab entries. Finite z of any size
+ * weigh by their distance to the largest. A row whose largest z is infinite, or
+ * that holds a NaN, has NaN log probabilities and entropy and rank -1 (among
+ * the top k a NaN logit counts as -inf). n is below
  * 2^24, vocab at most 2^30. workspace: 256-byte aligned, at least
  * dsv4g_logprobs_workspace_bytes(vocab, n, k) (0: none is needed, and it may
  * be NULL); a call uses nothing that an earlier one left there. No

@@ -177,3 +177,37 @@ def test_graph_and_streams(env):
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(b, want))
     assert all(torch.equal(x, y) for x, y in zip(a[3:], lib.logprobs(other, None, top=4)[3:]))
+
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [3, 2050], ids=["segments", "whole rows"])
+def test_values_of_any_size(env, kind, n):
+    """Masks of every size beside ordinary logits, rows of nothing but masks (of
+    one size, of two), largest values up to the end of fp32's range: a value
+    is as far from the largest as its difference says."""
+    torch, dev = env["torch"], env["dev"]
+    t = getattr(torch, kind)
+    v, low = 9001, torch.finfo(t).min
+    g = torch.Generator(device=dev).manual_seed(13)
+    some = torch.randn(v, generator=g, device=dev) * 3
+    first = torch.arange(v, device=dev) < 4500   # whole segments and places of a thread
+    third = torch.arange(v, device=dev) % 3 == 0
+    one = torch.arange(v, device=dev) == 8000
+    rows = []
+    for m in (-1e4, -1e6, -1e9, -1e10, -3e10, -1e20, -1e30, -1e37, -1e38, -3e38, low):
+        rows += [torch.where(first, m, some), torch.where(third, some, m),
+                 torch.where(one, some, m), torch.full_like(some, m),
+                 torch.where(third, m, low), torch.where(one, m, 3 * m if m > -1e38 else low)]
+    for m in (1e6, 1.7e7, 1e9, 1e10, 1e30, 2.3e38, 3e38):
+        rows += [torch.where(one, m, some), torch.full_like(some, m), torch.where(third, m, -m),
+                 torch.where(third, m, 0.999 * m), some + m]
+    # fp32 and BF16 steps around one large value
+    rows += [torch.where(third, 4e9, 4e9 - 256), torch.where(first, 1.7e7, 1.7e7 - 1)]
+    rows = torch.stack(rows).to(t)
+    tokens = [(0, 8000, 4501, 3, 9000)[i % 5] for i in range(len(rows))]
+    for i in range(0, len(rows), n):
+        z, tok = rows[i:i + n], tokens[i:i + n]
+        more = n - len(z) if n > len(rows) else 0   # fill the call with copies
+        check(env, torch.cat([z, z[:1].expand(more, v)]), tok + tok[:1] * more, 5, 1.0,
+              rows=range(len(z)))
+    check(env, rows[:n], tokens[:n], 0, 0.7)
