@@ -72,10 +72,11 @@ struct ScoreArgs {
   uint64_t *keys;   // [n][nseg][k]
 };
 
-// -0 counts as 0 and NaN as -inf in the order of values.
+// -0 counts as 0 (a product that vanishes keeps its sign) and NaN as -inf in the
+// order of values.
 __device__ __forceinline__ uint32_t ordered(float z) {
   if (z != z) z = -__builtin_inff();
-  const uint32_t u = f2u(z);
+  const uint32_t u = f2u(z + 0.0f);
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t o) {
@@ -232,7 +233,7 @@ struct Tile {
     T e[V];
     __builtin_memcpy(e, &raw[j / V], 16);
     const float f = sizeof(T) == 4 ? u2f((uint32_t)e[j % V]) : u2f((uint32_t)e[j % V] << 16);
-    return fmaf(f, scale, 0.0f);  // + 0: -0 becomes 0
+    return f * scale;
   }
   __device__ __forceinline__ static int place(int j) {
     return (j / V) * (SC_T * V) + V * threadIdx.x + j % V;
@@ -283,9 +284,9 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
   float zt = __builtin_nanf("");  // no logit is above it
   if (have) {
     const T e = l[token];
-    zt = fmaf(sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16), a.scale, 0.0f);
+    zt = (sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16)) * a.scale;
   }
-  // the next value below it (no z is -0)
+  // the next value below it: below 0 that is behind -0, which no order holds
   const float zt_below = unordered(ordered(zt) - (zt == 0.0f ? 2 : 1));
   if (TOP) {
     if (tid < 4) s_bar[tid] = -__builtin_inff();
@@ -433,7 +434,7 @@ __global__ __launch_bounds__(SC_T) void k_score_join(ScoreArgs a) {
   float zt = 0.0f;
   if (have) {
     const T e = ((const T *)a.logits)[(size_t)row * a.stride + token];
-    zt = fmaf(sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16), a.scale, 0.0f);
+    zt = (sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16)) * a.scale;
   }
   TopList top;
   top.init();

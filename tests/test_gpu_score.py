@@ -211,3 +211,26 @@ def test_values_of_any_size(env, kind, n):
         check(env, torch.cat([z, z[:1].expand(more, v)]), tok + tok[:1] * more, 5, 1.0,
               rows=range(len(z)))
     check(env, rows[:n], tokens[:n], 0, 0.7)
+
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [3, 2050], ids=["segments", "whole rows"])
+def test_products_that_vanish(env, kind, n):
+    """Logits whose products with the scale round to zero, of either sign: they
+    are equal, and go by their index."""
+    torch, dev = env["torch"], env["dev"]
+    t = getattr(torch, kind)
+    tiny = torch.nextafter(torch.zeros((), dtype=t), torch.ones((), dtype=t)).item()
+    some = torch.tensor([0.0, -0.0, tiny, -tiny, 3 * tiny, -3 * tiny], dtype=t, device=dev)
+    v = 2 * 4096 + 77
+    g = torch.Generator(device=dev).manual_seed(14)
+    # 2^-151, 0.75 2^-149 and the like: zero, and one last place of the least number
+    for scale in ((0.25, 0.75, 0.4) if kind == "float32" else (2.0 ** -18, 0.75 * 2.0 ** -16)):
+        z = some[torch.randint(0, 6, (n, v), generator=g, device=dev)]
+        z[1] = -tiny
+        z[1, 100:] = -0.0
+        z[2] = -tiny
+        tokens = [(4096 * (r % 3) + [0, 50, 4000, 76][r // 3 % 4]) % v for r in range(n)]
+        z[torch.arange(n, device=dev), torch.tensor(tokens, device=dev)] = \
+            some[torch.arange(n, device=dev) % 6]
+        check(env, z, tokens, 20, scale, rows=[r for r in range(36) if r < n])
