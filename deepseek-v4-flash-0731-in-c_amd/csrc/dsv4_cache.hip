@@ -343,13 +343,20 @@ __global__ __launch_bounds__(256) void k_cache_append(DSV4GCache C, CacheGeom G,
   const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   if (row >= n_tokens || *C.status) return;
   // starts[0] <= .. <= starts[n]: the sequence is the number of starts at or
-  // before the row, less one
+  // before the row, less one. Starts that fall somewhere place no row.
   int b = -1;
+  bool falls = false;
   for (int j = 0; j <= n; j += 64) {
     const int at = j + lane;
-    b += __popcll(__ballot(at <= n && starts[at] <= row));
+    const int from = at <= n ? starts[at] : 0x7FFFFFFF;
+    b += __popcll(__ballot(from <= row));
+    falls |= __ballot(at < n && starts[at + 1] < from) != 0;
   }
-  if (b < 0 || b >= n) return;  // in front of the first sequence or behind the last
+  // entries that reach out of the call's rows are reported by the first row:
+  // they may have none
+  const bool out = row == 0 && (starts[0] < 0 || starts[n] > n_tokens);
+  if ((falls || out) && lane == 0) atomicOr(C.status, DSV4G_CACHE_LIST);
+  if (falls || b < 0 || b >= n) return;  // b: in front of the first sequence or behind the last
   const int s = seqs ? seqs[b] : b;
   bool twice = false;
   if (seqs)
@@ -357,11 +364,13 @@ __global__ __launch_bounds__(256) void k_cache_append(DSV4GCache C, CacheGeom G,
       const int at = j + lane;
       twice |= __ballot(at < n && at != b && seqs[at] == s) != 0;
     }
+  // the whole entry is good or none of its rows is written
   int pos = -1;
   if (s >= 0 && s < C.n_seqs && !twice) {
-    const int end = starts[b + 1];
-    pos = C.len[s] - end + row;
-    if (starts[b] > row || end <= row || pos >= (long)C.max_pages * C.page_size) pos = -1;
+    const int first = starts[b], end = starts[b + 1], len = C.len[s];
+    if (first >= 0 && end <= n_tokens && len >= end - first &&
+        len <= (long)C.max_pages * C.page_size)
+      pos = len - end + row;
   }
   if (pos < 0) {
     if (lane == 0) atomicOr(C.status, DSV4G_CACHE_LIST);

@@ -442,8 +442,11 @@ int dsv4g_cache_reserve(const DSV4GCache *C, const int *seqs, const int *starts,
  * act_dtype DSV4G_DT_F32 or _BF16, 16-byte aligned rows. BF16 pages: rounded to
  * nearest even. E4M3 pages: the scale is the power of two that the activation
  * quantisation takes (2^ceil(log2(max(amax, 1e-4) / 448)), over the group's
- * finite values), codes to nearest even; infinities are held as NaN. A
- * sequence listed twice is not written. */
+ * finite values), codes to nearest even; infinities are held as NaN. Nothing of
+ * an entry is written whose sequence is listed twice or holds fewer tokens than
+ * it lists, or whose rows lie outside 0 .. n_tokens - 1; of the whole call,
+ * where starts fall. A table entry that is no page takes the rows of that page
+ * with it. */
 int dsv4g_cache_append(const DSV4GCache *C, int layer, const void *k, size_t k_stride,
                        const void *v, size_t v_stride, int act_dtype, const int *seqs,
                        const int *starts, int n_seqs, int n_tokens, void *stream);

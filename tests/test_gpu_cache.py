@@ -282,3 +282,67 @@ def test_bookkeeping_in_a_graph(env):
         check(env, c, book, moved(image, moves))
         lib.cache_free(c, kids)
         (c.pages.float().sum() * i).item()
+
+
+def rows(env, n, c, seed):
+    """New tokens' keys and values for a cache, float32."""
+    torch, s = env["torch"], c.struct
+    g = torch.Generator(device=env["dev"]).manual_seed(seed)
+    return [torch.randn(n, s.kv_heads, d, generator=g, device=env["dev"]) if d else None
+            for d in (s.k_dim, s.v_dim)]
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[1]], ids=str)
+def test_append_skips_whole_entries(env, shape):
+    """An entry with more new tokens than its sequence holds, with rows outside
+    the call's or with a length beyond its table, one listed twice: none of
+    its rows is written, pages shared with a fork among them, and the entries
+    beside it are as in a call without it."""
+    torch, lib = env["torch"], env["lib"]
+    c, book = new_cache(env, shape)
+    lib.cache_reserve(c, starts_of(env, [40, 70, 9]), ints(env, [0, 1, 2]))
+    lib.cache_fork(c, ints(env, [0]), ints(env, [5]))
+    assert lib.cache_status(c) == 0
+    clean = c.pages.clone()
+    k, v = rows(env, 120, c, 4)
+
+    def call(seqs, starts, n=120):
+        lib.cache_append(c, 1, k[:n], None if v is None else v[:n], ints(env, starts),
+                         ints(env, seqs))
+
+    def reset():
+        c.pages.copy_(clean)
+
+    for seqs, starts, good, good_starts, n in (
+            ([0], [0, 41], None, None, 120),              # more than it holds
+            ([5, 1], [0, 41, 111], [1], [41, 111], 120),
+            ([1, 0], [3, 10, 90], [1], [3, 10], 120),
+            ([0, 0], [0, 5, 9], None, None, 120),         # twice
+            ([2, 0, 1, 0], [0, 9, 20, 60, 61], [2, 1], [0, 9], 120),
+            ([1, 2], [0, 20, 29], [1], [0, 20], 25),      # its end behind the rows
+            ([1, 2], [0, 20, 29], [1], [0, 20], 20),      # all of it
+            ([2, 1], [-3, 6, 50], [1], [6, 50], 120),     # its start before them
+            ([2, 1], [-9, 0, 50], [1], [0, 50], 120),
+            ([-1, 1], [0, 4, 50], [1], [4, 50], 120), ([9, 1], [0, 4, 50], [1], [4, 50], 120),
+            ([3, 1], [0, 4, 50], [1], [4, 50], 120),      # holds nothing
+            ([1, 2], [10, 5, 14], None, None, 120),       # starts that fall
+            ([1, 2, 0], [0, 20, 10, 30], None, None, 120)):
+        reset()
+        if good:
+            if seqs[0] == 2 and len(seqs) == 4:           # the good ones are not neighbours
+                call([2], [0, 9])
+                call([1], [20, 60])
+            else:
+                call(good, good_starts, n)
+            assert lib.cache_status(c) == 0
+        want = c.pages.clone()
+        reset()
+        call(seqs, starts, n)
+        assert lib.cache_status(c) == LIST, (seqs, starts)
+        assert torch.equal(c.pages, want), (seqs, starts)
+    for length in (-1, 12 * shape[0] + 1, 2 ** 31 - 1):
+        reset()
+        c.length[2] = length
+        call([2], [0, 1])
+        assert lib.cache_status(c) == LIST
+        assert torch.equal(c.pages, clean)
