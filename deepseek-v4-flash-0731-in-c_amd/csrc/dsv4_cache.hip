@@ -15,6 +15,13 @@
 
 namespace dsv4 {
 
+// An append may neither wait for its other waves nor be stopped by what they
+// report: it sets its bits one byte up, and is blocked by those of the lowest.
+constexpr int CACHE_APPEND = DSV4G_CACHE_BY_APPEND;
+__host__ __device__ inline unsigned cache_bits(unsigned status) {
+  return (status | status >> CACHE_APPEND) & ((1u << CACHE_APPEND) - 1);
+}
+
 constexpr int CB_T = 1024;  // threads of a deciding workgroup (and most listed sequences)
 constexpr int CB_PER = 8;   // refs per thread and step of a scan over the pool
 static_assert(CB_T == DSV4G_CACHE_MAX_SEQS, "one thread per listed sequence");
@@ -79,7 +86,13 @@ __global__ __launch_bounds__(CB_T) void k_cache_reserve(DSV4GCache C, const int 
   const CacheWs w = cache_ws(ws, C.n_pages);
   const int t = threadIdx.x;
   if (t == 0) w.head[0] = 0;
-  if (*C.status) return;  // the same word for every thread: nothing here has written yet
+  const unsigned status = *C.status;  // not 0 for every thread, or for none
+  if (status) {
+    // appends of the step that was refused are over: from here on their
+    // refusals block appends, too
+    if (t == 0) *C.status = cache_bits(status);
+    return;
+  }
   const int ps = C.page_size, room = C.max_pages;
   int s = -1, count = 0, L = 0, P = -1, full = 0;
   bool bad = false, bad_page = false;
@@ -341,7 +354,8 @@ __global__ __launch_bounds__(256) void k_cache_append(DSV4GCache C, CacheGeom G,
                                                       int n_tokens) {
   const int lane = threadIdx.x % 64;
   const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  if (row >= n_tokens || *C.status) return;
+  // of earlier calls: waves of this one set others
+  if (row >= n_tokens || (*C.status & ((1u << CACHE_APPEND) - 1))) return;
   // starts[0] <= .. <= starts[n]: the sequence is the number of starts at or
   // before the row, less one. Starts that fall somewhere place no row.
   int b = -1;
@@ -355,7 +369,7 @@ __global__ __launch_bounds__(256) void k_cache_append(DSV4GCache C, CacheGeom G,
   // entries that reach out of the call's rows are reported by the first row:
   // they may have none
   const bool out = row == 0 && (starts[0] < 0 || starts[n] > n_tokens);
-  if ((falls || out) && lane == 0) atomicOr(C.status, DSV4G_CACHE_LIST);
+  if ((falls || out) && lane == 0) atomicOr(C.status, DSV4G_CACHE_LIST << CACHE_APPEND);
   if (falls || b < 0 || b >= n) return;  // b: in front of the first sequence or behind the last
   const int s = seqs ? seqs[b] : b;
   bool twice = false;
@@ -373,12 +387,12 @@ __global__ __launch_bounds__(256) void k_cache_append(DSV4GCache C, CacheGeom G,
       pos = len - end + row;
   }
   if (pos < 0) {
-    if (lane == 0) atomicOr(C.status, DSV4G_CACHE_LIST);
+    if (lane == 0) atomicOr(C.status, DSV4G_CACHE_LIST << CACHE_APPEND);
     return;
   }
   const int page = C.table[(size_t)s * C.max_pages + (pos >> G.shift)];
   if (page < 0 || page >= C.n_pages) {
-    if (lane == 0) atomicOr(C.status, DSV4G_CACHE_PAGE);
+    if (lane == 0) atomicOr(C.status, DSV4G_CACHE_PAGE << CACHE_APPEND);
     return;
   }
   uint8_t *base = C.pages + ((size_t)layer * C.n_pages + page) * G.page_bytes;
@@ -510,6 +524,7 @@ int dsv4g_cache_status(unsigned *status_out, const DSV4GCache *C, void *stream) 
   if (*status_out) {
     hipLaunchKernelGGL(k_cache_clear_status, dim3(1), dim3(1), 0, st, C->status);
     DSV4G_TRY(dsv4g_check_launch("cache_status"));
+    *status_out = cache_bits(*status_out);
   }
   return 0;
 }

@@ -403,13 +403,17 @@ int dsv4g_ffn_step(float *state, const float *hc_fn, const float *hc_scale,
  * the sticky *status. While *status is not 0, dsv4g_cache_reserve, _append and
  * dsv4g_attention do nothing (their outputs are left as they were), so that no
  * later call of an engine's queue works on a cache that the refused call did
- * not prepare. dsv4g_cache_status reads and clears it. Calls on one cache
- * must be ordered (one stream, or events). */
+ * not prepare. An append's own bits stand DSV4G_CACHE_BY_APPEND higher in
+ * *status until a reserve has met them: they do not block the appends in
+ * between, and what an append writes beside a refused entry is whole.
+ * dsv4g_cache_status reads and clears the word, all bits in their place. Calls
+ * on one cache must be ordered (one stream, or events). */
 #define DSV4G_CACHE_GROUP 64
 #define DSV4G_CACHE_MAX_SEQS 1024 /* listed in one _reserve, _fork or _free */
 #define DSV4G_CACHE_FULL 1u       /* *status: fewer free pages than reserve needed */
 #define DSV4G_CACHE_LIST 2u       /* a listed sequence, count or length that cannot be */
 #define DSV4G_CACHE_PAGE 4u       /* a table entry that is no page */
+#define DSV4G_CACHE_BY_APPEND 8   /* shift of these bits where append set them */
 typedef struct {
     uint8_t *pages;   /* device, 256-byte aligned: [n_layers][n_pages][page_bytes] */
     int *ref;         /* device [n_pages] */

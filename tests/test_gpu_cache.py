@@ -346,3 +346,46 @@ def test_append_skips_whole_entries(env, shape):
         call([2], [0, 1])
         assert lib.cache_status(c) == LIST
         assert torch.equal(c.pages, clean)
+
+
+@pytest.mark.parametrize("bad", ["list", "page"])
+def test_append_writes_what_stands_beside_a_refused_entry(env, bad):
+    """Thousands of valid tokens behind a refused entry, in several layers: all
+    of them are written whatever waves of the call have met it, and so in
+    the appends that follow; reserve, append and attention are blocked as soon
+    as a reserve has met the refusal, until the status is read."""
+    torch, lib = env["torch"], env["lib"]
+    c, book = new_cache(env, (16, 1, 64, 64, False), layers=3, pages=1100, seqs=5, cols=500)
+    counts, seqs = [33, 4000, 5000, 7000], [0, 1, 2, 3]
+    lib.cache_reserve(c, starts_of(env, counts), ints(env, seqs))
+    book.reserve(seqs, counts)
+    k, v = rows(env, sum(counts), c, 5)
+    starts = starts_of(env, counts)
+    if bad == "page":
+        c.table[0, 1:] = 5000
+    else:
+        lib.cache_free(c, ints(env, [0]), ints(env, [20]))
+        book.free([0], [20])
+    assert lib.cache_status(c) == 0
+    clean = c.pages.clone()
+    for layer in range(3):  # the valid ones alone
+        lib.cache_append(c, layer, k, v, starts[1:].contiguous(), ints(env, seqs[1:]))
+    want = c.pages.clone()
+    for _ in range(5):
+        c.pages.copy_(clean)
+        for layer in range(3):
+            lib.cache_append(c, layer, k, v, starts, ints(env, seqs))
+        got = c.pages.clone()
+        if bad == "page":  # the rows that its first page takes
+            got[:, book.table[0][0]] = want[:, book.table[0][0]]
+        assert torch.equal(got, want)
+        image = c.pages.clone()
+        out = torch.full((3, 2, 64), 7.0, dtype=torch.bfloat16, device=env["dev"])
+        st = ints(env, [0, 3])
+        lib.attention(c, 0, out.clone(), st, ints(env, [1]), out=out)
+        lib.cache_reserve(c, st, ints(env, [1]))
+        lib.cache_append(c, 1, k, v, starts[1:].contiguous(), ints(env, [3, 2, 1]))
+        assert (out == 7).all() and c.length.tolist() == book.len
+        assert torch.equal(c.pages, image)
+        assert lib.cache_status(c) == (PAGE if bad == "page" else LIST)
+    assert lib.cache_status(c) == 0
