@@ -157,9 +157,10 @@ struct Item {
   int b, kvh, seq, start, count, len, r0, nrows, lo, hi, clear, stages;
 };
 // Rows tile * ROWS .. of the b-th listed sequence; false: there are none.
+// blocked: by an earlier refusal, which stays the only one reported.
 template <int ROWS, int TT>
 __device__ __forceinline__ bool attn_item(const DSV4GCache &C, const AttnArgs &a, int b, int tile,
-                                          Item &it) {
+                                          unsigned blocked, Item &it) {
   it.b = b;
   it.seq = a.seqs ? a.seqs[b] : b;
   it.start = a.starts[b];
@@ -168,7 +169,7 @@ __device__ __forceinline__ bool attn_item(const DSV4GCache &C, const AttnArgs &a
   it.len = it.seq >= 0 && it.seq < C.n_seqs ? C.len[it.seq] : -1;
   if (it.start < 0 || end > a.n_tokens || count < 0 || count > a.max_q || it.len < count ||
       it.len > a.max_kv || it.len > (long)C.max_pages * C.page_size) {
-    if (tile == 0) atomicOr(C.status, DSV4G_CACHE_LIST);
+    if (tile == 0 && !blocked) atomicOr(C.status, DSV4G_CACHE_LIST);
     return false;
   }
   it.count = (int)count;
@@ -223,7 +224,8 @@ struct Place {
   Item it;  // of the first pair
 };
 template <int ROWS, int TT>
-__device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &a, Place &p) {
+__device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &a,
+                                           unsigned blocked, Place &p) {
   __shared__ long s_sum[4];
   __shared__ int s_at[3];
   __shared__ Item s_item;
@@ -233,7 +235,8 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
   long mine = 0;
   Item it;
   for (int j = j0; j < j1; ++j)
-    if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, it)) mine += it.stages + AT_START;
+    if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, blocked, it))
+      mine += it.stages + AT_START;
   long x = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -258,7 +261,7 @@ __device__ __forceinline__ void attn_place(const DSV4GCache &C, const AttnArgs &
   p.end = share_begin(p.total, groups, blockIdx.x + 1);
   if (p.at >= before && p.at < before + mine * C.kv_heads)
     for (int j = j0; j < j1; ++j)
-      if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, it)) {
+      if (attn_item<ROWS, TT>(C, a, j / a.tiles, j % a.tiles, blocked, it)) {
         const int span = it.stages + AT_START;
         const long all = (long)span * C.kv_heads;
         if (p.at < before + all) {
@@ -663,7 +666,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
 
   Place w;
   if (a.groups) {
-    attn_place<F::ROWS, TT>(C, a, w);
+    attn_place<F::ROWS, TT>(C, a, bad, w);
   } else {
     int id = blockIdx.x;
     w.kvh = id % C.kv_heads;
@@ -681,7 +684,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     Item it;
     if (first && a.groups) {
       it = w.it;  // looked up already
-    } else if (!attn_item<F::ROWS, TT>(C, a, w.pair / a.tiles, w.pair % a.tiles, it)) {
+    } else if (!attn_item<F::ROWS, TT>(C, a, w.pair / a.tiles, w.pair % a.tiles, 0, it)) {
       if (!a.groups) return;
       ++w.pair;  // no rows here
       continue;
@@ -1036,7 +1039,7 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
   const int kvh = id % C.kv_heads, pair = id / C.kv_heads;
   const long total = a.first[0], at = a.first[1 + id];
   Item it;
-  if (bad || !attn_item<ROWS, TT>(C, a, pair / a.tiles, pair % a.tiles, it)) return;
+  if (bad || !attn_item<ROWS, TT>(C, a, pair / a.tiles, pair % a.tiles, 0, it)) return;
   const int groups = shared_groups(a, total);
   if (groups <= 0) return;
   const int w0 = max(0, share_of(total, groups, at));

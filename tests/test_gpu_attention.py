@@ -586,3 +586,22 @@ def test_single_tokens_with_large_scores(env):
         # 512 exact products summed in fp32, scaled once more
         tol = 520 * 2.0 ** -24 * (q.double() * keys).abs().sum(2) + 1e-6
         assert ((lse.double() - z).abs() <= tol).all(), size
+
+
+@pytest.mark.parametrize("shape", [LATENT, GQA], ids=str)
+@pytest.mark.parametrize("kv", [64, 65536], ids=["whole", "dealt out"])
+def test_a_blocked_call_adds_no_status(env, shape, kv):
+    """A pool without room for a new sequence: the attention that follows leaves
+    the refusal as it is, though the sequence holds less than it is to have."""
+    torch, lib, dev = env["torch"], env["lib"], env["dev"]
+    heads, kvh, kd, vd = shape
+    c = env["gpu"].PagedCache.new(1, 4, 16, kvh, kd, vd, 2, 4096, "bf16", dev)
+    lib.cache_reserve(c, ints(env, [0, 40]), ints(env, [0]))
+    starts = ints(env, [0, 1, 31])
+    assert (lib.attention_workspace_bytes(c, heads, 2, 31, 30, kv) > 0) == (kv > 64)
+    lib.cache_reserve(c, starts)
+    q = torch.zeros(31, heads, kd, dtype=torch.bfloat16, device=dev)
+    out = torch.full((31, heads, vd or kd), 5.0, dtype=torch.bfloat16, device=dev)
+    lib.attention(c, 0, q, starts, max_q=30, max_kv=kv, out=out)
+    assert lib.cache_status(c) == paged.FULL
+    assert (out == 5).all() and c.length.tolist() == [40, 0]
