@@ -227,7 +227,16 @@ __global__ __launch_bounds__(256) void k_cache_move(DSV4GCache C, int *ws, size_
   }
 }
 
-// Whether listed sequence i's partner conflicts: child named twice, or a parent.
+// Whether entries from .. to - 1 of a sequence's row name pages, for all
+// threads of the workgroup; a barrier.
+__device__ __forceinline__ bool pages_good(const DSV4GCache &C, const int *row, int from, int to) {
+  bool bad = false;
+  for (int k = from + threadIdx.x; k < to; k += 256) bad |= row[k] < 0 || row[k] >= C.n_pages;
+  return !__syncthreads_or(bad);
+}
+
+// A workgroup per pair, which first looks for what conflicts: a child named
+// twice or as a parent, lengths, entries of the parent that are no pages.
 __global__ __launch_bounds__(256) void k_cache_fork(DSV4GCache C, const int *parents,
                                                     const int *children, int n) {
   const int i = blockIdx.x, t = threadIdx.x;
@@ -247,12 +256,14 @@ __global__ __launch_bounds__(256) void k_cache_fork(DSV4GCache C, const int *par
   const int held = (L + C.page_size - 1) / C.page_size;
   const int *from = C.table + (size_t)p * C.max_pages;
   int *to = C.table + (size_t)c * C.max_pages;
+  if (!pages_good(C, from, 0, held)) {
+    if (t == 0) atomicOr(C.status, DSV4G_CACHE_PAGE);
+    return;
+  }
   for (int k = t; k < C.max_pages; k += 256) {
     const int e = k < held ? from[k] : -1;
     to[k] = e;
-    if (k >= held) continue;
-    if (e >= 0 && e < C.n_pages) atomicAdd(&C.ref[e], 1);
-    else atomicOr(C.status, DSV4G_CACHE_PAGE);
+    if (k < held) atomicAdd(&C.ref[e], 1);
   }
   if (t == 0) C.len[c] = L;
 }

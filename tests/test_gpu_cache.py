@@ -389,3 +389,24 @@ def test_append_writes_what_stands_beside_a_refused_entry(env, bad):
         assert torch.equal(c.pages, image)
         assert lib.cache_status(c) == (PAGE if bad == "page" else LIST)
     assert lib.cache_status(c) == 0
+
+
+def test_fork_skips_a_parent_with_a_bad_entry(env):
+    """A parent whose table names no page: its child stays empty and no page's
+    count changes; the other pairs of the list are forked."""
+    lib = env["lib"]
+    c, book = new_cache(env, SHAPES[1])
+    lib.cache_reserve(c, starts_of(env, [100, 70]), ints(env, [0, 1]))
+    book.reserve([0, 1], [100, 70])
+    for entry in (-1, 40, 2 ** 31 - 1, -2 ** 31):
+        for at in (0, 3):
+            good = book.table[0][at]
+            c.table[0, at] = book.table[0][at] = entry
+            lib.cache_fork(c, ints(env, [0, 1, 0]), ints(env, [4, 5, 6]))
+            book.fork([1], [5])
+            book.status = PAGE
+            check(env, c, book, None)
+            c.table[0, at] = book.table[0][at] = good
+            lib.cache_free(c, ints(env, [5]))
+            book.free([5], [0])
+            check(env, c, book, None)
