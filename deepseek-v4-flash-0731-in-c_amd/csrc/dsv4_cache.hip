@@ -284,13 +284,15 @@ __global__ __launch_bounds__(256) void k_cache_free(DSV4GCache C, const int *seq
     if (t == 0) atomicOr(C.status, DSV4G_CACHE_LIST);
     return;
   }
-  const int ps = C.page_size, held = (L + ps - 1) / ps;
+  const int ps = C.page_size, held = (L + ps - 1) / ps, kept = (to + ps - 1) / ps;
   int *row = C.table + (size_t)s * C.max_pages;
-  for (int k = (to + ps - 1) / ps + t; k < held; k += 256) {
-    const int e = row[k];
+  if (!pages_good(C, row, kept, held)) {
+    if (t == 0) atomicOr(C.status, DSV4G_CACHE_PAGE);
+    return;
+  }
+  for (int k = kept + t; k < held; k += 256) {
+    atomicSub(&C.ref[row[k]], 1);
     row[k] = -1;
-    if (e >= 0 && e < C.n_pages) atomicSub(&C.ref[e], 1);
-    else atomicOr(C.status, DSV4G_CACHE_PAGE);
   }
   if (t == 0) C.len[s] = to;
 }

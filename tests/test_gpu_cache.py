@@ -410,3 +410,32 @@ def test_fork_skips_a_parent_with_a_bad_entry(env):
             lib.cache_free(c, ints(env, [5]))
             book.free([5], [0])
             check(env, c, book, None)
+
+
+def test_free_skips_a_sequence_with_a_bad_entry(env):
+    """A sequence whose table names no page behind the cut: its length, its row
+    and the pages' counts stay as they were; the others of the list are cut.
+    Entries in front of the cut are not looked at."""
+    lib = env["lib"]
+    c, book = new_cache(env, SHAPES[1])
+    lib.cache_reserve(c, starts_of(env, [100, 70]), ints(env, [0, 1]))
+    book.reserve([0, 1], [100, 70])
+    for entry in (-1, 40, 2 ** 31 - 1, -2 ** 31):
+        for at in (1, 3):
+            good = book.table[0][at]
+            c.table[0, at] = book.table[0][at] = entry
+            lib.cache_fork(c, ints(env, [1]), ints(env, [5]))
+            book.fork([1], [5])
+            lib.cache_free(c, ints(env, [0, 5]), ints(env, [32, 32]))
+            book.free([5], [32])
+            book.status = PAGE
+            check(env, c, book, None)
+            lib.cache_free(c, ints(env, [5]))
+            book.free([5], [0])
+            c.table[0, at] = book.table[0][at] = good
+            check(env, c, book, None)
+    good = book.table[0][0]
+    c.table[0, 0] = book.table[0][0] = -1
+    lib.cache_free(c, ints(env, [0]), ints(env, [40]))
+    book.free([0], [40])
+    check(env, c, book, None)
