@@ -483,7 +483,7 @@ extern "C" {
 
 size_t dsv4g_cache_page_bytes(const DSV4GCache *C) {
   CacheGeom G;
-  return cache_geom(C, &G) ? G.page_bytes : 0;
+  return C && cache_geom(C, &G) ? G.page_bytes : 0;
 }
 
 // The descriptor's own checks, for every entry that takes one.

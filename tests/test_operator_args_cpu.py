@@ -198,3 +198,20 @@ def test_scales_beyond_fp32_in_base_2(raw):
         assert raw.dsv4g_attention(P, a["os"], P, P, a["qs"], BF16, c, 1, 8, P, P, 2, 5, 5, 8192,
                                    scale, 0, P, P, 0, None) == 1
         assert why in raw.dsv4g_last_error(), scale
+
+
+def test_no_descriptor(raw):
+    """NULL in place of the descriptor: no size, and a refusal."""
+    assert raw.dsv4g_cache_page_bytes(None) == 0
+    assert raw.dsv4g_cache_workspace_bytes(None) == 0
+    assert raw.dsv4g_attention_workspace_bytes(None, 8, 2, 5, 5, 100) == 0
+    a = GOOD_ATT
+    for rc in (raw.dsv4g_cache_init(None, None), raw.dsv4g_cache_fork(None, P, P, 1, None),
+               raw.dsv4g_cache_reserve(None, P, P, 2, P, 1 << 20, None),
+               raw.dsv4g_cache_append(None, 0, P, 256, P, 256, F32, P, P, 2, 5, None),
+               raw.dsv4g_cache_free(None, P, P, 2, None),
+               raw.dsv4g_cache_compact(None, P, P, 1 << 20, None),
+               raw.dsv4g_cache_status(P, None, None),
+               raw.dsv4g_attention(P, a["os"], P, P, a["qs"], BF16, None, 1, 8, P, P, 2, 5, 5, 100,
+                                   0.1, 0, P, P, 1 << 30, None)):
+        assert rc == 1 and b"cache shape" in raw.dsv4g_last_error()
