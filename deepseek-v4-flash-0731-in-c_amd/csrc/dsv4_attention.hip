@@ -1131,7 +1131,7 @@ __global__ __launch_bounds__(256) void k_attn_join(DSV4GCache C, AttnArgs a) {
 // ------------------------------------------------------------- launch plan
 struct AttnPlan {
   int rw, tiles, groups;
-  long items;
+  long items;  // 0: more than a launch takes
   size_t bytes;
 };
 template <int D, bool SHARED>
@@ -1144,7 +1144,7 @@ static int attn_places(int rw, bool fp8) {  // workgroups that the chip holds
 // item only gets shorter.
 static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_tokens, int max_q,
                           int max_kv, int window) {
-  AttnPlan p;
+  AttnPlan p = {};
   max_q = max_q > n_tokens ? n_tokens : max_q;
   const int group = heads / C->kv_heads;
   const long rows = (long)max_q * group;
@@ -1153,8 +1153,13 @@ static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_toke
   const int least = D == 512 || (D == 256 && C->v_dim) ? 2 : 1;
   p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   p.rw = p.rw < least ? least : p.rw;
+  // a launch is below 2^32 threads, a sequence's rows (new tokens * heads of a
+  // kv head) below 2^31; each product only once the one before is known to fit
+  if (rows > 0x7FFFFF00L) return p;
   p.tiles = (int)((rows + 32 * p.rw - 1) / (32 * p.rw));
-  p.items = (long)p.tiles * n_seqs * C->kv_heads;
+  const long pairs = (long)p.tiles * n_seqs;
+  if (pairs > 0xFFFFFFL || pairs * C->kv_heads > 0xFFFFFFL) return p;
+  p.items = pairs * C->kv_heads;
   const bool fp8 = C->dtype == DSV4G_DT_F8_E4M3;
   const int places = D == 64    ? attn_places<64, false>(p.rw, fp8)
                      : D == 128 ? attn_places<128, false>(p.rw, fp8)
@@ -1176,7 +1181,6 @@ static AttnPlan attn_plan(const DSV4GCache *C, int heads, int n_seqs, int n_toke
   const double idle = std::max(std::ceil(r) - r, 0.5) * (S + AT_START);
   const double parts = p.rw * D / 64.0 * std::min(1.0, p.items * S / (2.0 * places));
   p.groups = r < 3 && idle > AT_START + 3 + parts ? places : 0;
-  p.bytes = 0;
   if (p.groups)
     p.bytes = (size_t)p.groups * 2 * 32 * p.rw * (D * sizeof(float) + sizeof(float2)) +
               (1 + (size_t)p.items) * sizeof(long);
@@ -1242,11 +1246,7 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
   // 32 bits
   if (window >= (long)C->max_pages * C->page_size) window = 0;
   const AttnPlan p = attn_plan(C, heads, n_seqs, n_tokens, max_q, max_kv, window);
-  // a launch is below 2^32 threads, a sequence's rows (new tokens * heads of a
-  // kv head) below 2^31
-  if (p.items > 0xFFFFFFL ||
-      (long)(max_q < n_tokens ? max_q : n_tokens) * (heads / C->kv_heads) > 0x7FFFFF00L)
-    return dsv4g_fail(DSV4G_EINVAL, "attention: too many rows for one call");
+  if (p.items == 0) return dsv4g_fail(DSV4G_EINVAL, "attention: too many rows for one call");
   if (p.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.bytes))
     return dsv4g_fail(DSV4G_EINVAL, "attention: 256-byte aligned workspace of %zu bytes needed "
                       "(%zu given)", p.bytes, workspace_bytes);

@@ -572,6 +572,8 @@ int dsv4g_cache_append(const DSV4GCache *C, int layer, const void *k, size_t k_s
     return dsv4g_fail(DSV4G_EINVAL, "cache_append: bad arguments");
   if (n_tokens > 0x3FFFFFF)  // a wave each, a launch is below 2^32 threads
     return dsv4g_fail(DSV4G_EINVAL, "cache_append: %d tokens, at most 2^26 - 1", n_tokens);
+  if (n_seqs > 0x3FFFFFF)  // counted in steps of a wave
+    return dsv4g_fail(DSV4G_EINVAL, "cache_append: %d sequences, at most 2^26 - 1", n_seqs);
   const size_t unit = act_dtype == DSV4G_DT_F32 ? 4 : 8;  // elements of 16 bytes
   if (k_stride < (size_t)C->kv_heads * C->k_dim || (v && v_stride < (size_t)C->kv_heads * C->v_dim) ||
       ((uintptr_t)k & 15) || ((uintptr_t)v & 15) || k_stride % unit || (v && v_stride % unit))

@@ -215,3 +215,20 @@ def test_no_descriptor(raw):
                raw.dsv4g_attention(P, a["os"], P, P, a["qs"], BF16, None, 1, 8, P, P, 2, 5, 5, 100,
                                    0.1, 0, P, P, 1 << 30, None)):
         assert rc == 1 and b"cache shape" in raw.dsv4g_last_error()
+
+
+def test_sizes_beyond_every_launch(raw):
+    """Products of sizes that pass 64 bits are refused as too many rows, and
+    take no workspace; the same for lists that no counter of the device holds."""
+    c, a = C.byref(cache(kv_heads=1024, k_dim=64, v_dim=64)), GOOD_ATT
+    for heads, n_seqs, tokens in ((1024, 1 << 30, 0x7FFFFF00), (1024, 1 << 29, 0x7FFFFF00),
+                                  (1024, 2**31 - 1, 1), (1 << 30, 1, 2**31 - 1),
+                                  (1 << 30, 2**31 - 1, 2**31 - 1)):
+        assert raw.dsv4g_attention_workspace_bytes(c, heads, n_seqs, tokens, tokens, 128) == 0
+        assert raw.dsv4g_attention(P, heads * 64, P, P, heads * 64, BF16, c, 1, heads, P, P,
+                                   n_seqs, tokens, tokens, 128, 0.1, 0, P, P, 1 << 62, None) == 1
+        assert b"too many rows" in raw.dsv4g_last_error(), (heads, n_seqs, tokens)
+    c = C.byref(cache())
+    for n in (1 << 26, 2**31 - 1):
+        assert raw.dsv4g_cache_append(c, 0, P, 256, P, 256, F32, P, P, n, 5, None) == 1
+        assert b"2^26" in raw.dsv4g_last_error()
