@@ -605,3 +605,20 @@ def test_a_blocked_call_adds_no_status(env, shape, kv):
     lib.attention(c, 0, q, starts, max_q=30, max_kv=kv, out=out)
     assert lib.cache_status(c) == paged.FULL
     assert (out == 5).all() and c.length.tolist() == [40, 0]
+
+
+@pytest.mark.parametrize("shape", [LATENT, SHARD, LAT256, GQA, ONE, ODD, WIDE, MHA], ids=str)
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_one_batch_under_both_plans(env, shape, fp8):
+    """A batch that takes no workspace under a close bound (its items are whole)
+    and one under a wide bound (its stages are dealt out)."""
+    lib = env["lib"]
+    past, new = [60, 0, 33, 71, 12], [2, 1, 0, 2, 2]
+    s = Setup(env, shape, 16, fp8, past, new, seed=17)
+    c, heads = wide_table(s), shape[0]
+    need = [lib.attention_workspace_bytes(c, heads, 5, 7, 2, kv) for kv in (73, 65536)]
+    assert need[0] == 0 and need[1] > 0
+    for kv in (73, 65536):
+        out, lse = lib.attention(c, 1, s.q, s.starts, max_q=2, max_kv=kv, with_lse=True)
+        s.check(out, lse)
+    assert lib.cache_status(c) == 0
