@@ -73,7 +73,11 @@ constexpr float AT_GROW = 8.0f;  // log2 of what the weights may grow to before 
 // A row's sums are kept against its m, the largest product q.k so far less what
 // it may have grown since: weights are 2^((z - m) c2). The difference comes
 // first: 2^(z c2 - fl(m c2)), one instruction less, would carry the rounding of
-// m c2, which no 2^x holds once scores pass 2^30.
+// m c2, which no 2^x holds once scores pass 2^30. With c2 below AT_TINY a
+// distance that no fp32 number holds has a weight: the queries are halved then
+// (what subnormal ones lose is far below a score's last place), and the scale is
+// doubled.
+constexpr float AT_TINY = 0x1p-100f;
 __device__ __forceinline__ float attn_c2(float scale) {
   // not 0: a hidden score stays -inf
   return fmaxf(fabsf(scale) * LOG2E, 1.4e-45f);
@@ -97,6 +101,7 @@ struct AttnArgs {
   float2 *stat;
   long *first;
   int layer, heads, group, n_seqs, n_tokens, max_q, max_kv, window, f32;
+  int halve;  // queries are halved, scale is doubled
   int tiles, groups;  // groups: workgroups that share the stages, or 0: one per item
   float scale;
 };
@@ -751,6 +756,11 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
         } else {
           u = *(const U4 *)((const uint16_t *)a.q + at + 16 * s);
         }
+        if (a.halve) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            u[k] = pack_bf16(0.5f * u2f(u[k] << 16), 0.5f * u2f(u[k] & 0xFFFF0000u));
+        }
         q[s] = __builtin_bit_cast(Bf8, u ^ sign);
       }
     }
@@ -1255,7 +1265,8 @@ int dsv4g_attention(void *out, size_t out_stride, float *lse, const void *q, siz
   a.seqs = seqs, a.starts = starts, a.sink = sink, a.layer = layer, a.heads = heads;
   a.group = heads / C->kv_heads, a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.max_q = max_q;
   a.max_kv = max_kv, a.window = window, a.f32 = act_dtype == DSV4G_DT_F32;
-  a.tiles = p.tiles, a.groups = p.groups, a.scale = scale;
+  a.tiles = p.tiles, a.groups = p.groups, a.halve = fabsf(scale) * LOG2E < AT_TINY;
+  a.scale = a.halve ? 2.0f * scale : scale;
   if (p.groups) {
     const size_t cells = (size_t)p.groups * 2 * 32 * p.rw;
     a.part = (float *)workspace;

@@ -622,3 +622,34 @@ def test_one_batch_under_both_plans(env, shape, fp8):
         out, lse = lib.attention(c, 1, s.q, s.starts, max_q=2, max_kv=kv, with_lse=True)
         s.check(out, lse)
     assert lib.cache_status(c) == 0
+
+
+@pytest.mark.parametrize("shape", [LATENT, LAT256, GQA, ONE, WIDE], ids=str)
+def test_products_at_both_ends_of_fp32(env, shape):
+    """Products near the largest number of either sign, whose difference no fp32
+    number holds, under scales that bring them close to each other."""
+    torch, lib, dev = env["torch"], env["lib"], env["dev"]
+    heads, kvh, kd, vd = shape
+    past, new = [300, 0, 33], [2, 1, 40]
+    s = Setup(env, shape, 16, False, past, new, seed=23)
+    sign = torch.randint(0, 2, (s.k.shape[0], kvh, 1), device=dev,
+                         generator=torch.Generator(device=dev).manual_seed(6)) * 2.0 - 1
+    s.k[:, :, 7:8] = 3.5 * sign
+    lib.cache_append(s.c, 1, s.k, s.v, ints(env, [0, 302, 303, 376]))
+    s.q.zero_()
+    s.q[:, :, 7] = 2.0 ** 126   # products of +-2.98e38
+    c = wide_table(s)
+    for scale in (0.0, 1e-38, -1e-38, 3e-39, 1e-37):
+        for kv in (302, 65536):
+            out, lse = lib.attention(c, 1, s.q, s.starts, max_q=40, max_kv=kv, scale=scale,
+                                     with_lse=True)
+            out, lse = out.double().cpu(), lse.double().cpu()
+            host, q = s.c.pages[1].cpu(), s.q.double().cpu()
+            for r, b in ((0, 0), (1, 0), (2, 1), (3, 2), (42, 2)):
+                held = paged.rows64(host, s.table[b], past[b] + new[b], 16, kvh, kd, vd, False)
+                o, e, mass = paged.attend64_far(q[r], *held, past[b] + r - s.starts[b].item(),
+                                                float(torch.tensor(scale, dtype=torch.float32)),
+                                                None)
+                tol, tol_lse = paged.attend_bounds(o, mass, torch.zeros_like(e), kd)
+                assert ((out[r] - o).abs() <= tol).all(), (scale, kv, r)
+                assert ((lse[r] - e).abs() <= tol_lse).all(), (scale, kv, r)
