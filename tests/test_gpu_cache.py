@@ -439,3 +439,57 @@ def test_free_skips_a_sequence_with_a_bad_entry(env):
     lib.cache_free(c, ints(env, [0]), ints(env, [40]))
     book.free([0], [40])
     check(env, c, book, None)
+
+
+def test_the_largest_lists(env):
+    """As many sequences as a list may name, in any order: forked, grown and cut
+    back together, and appended to; lists that are wrong at any place of it."""
+    torch, lib = env["torch"], env["lib"]
+    n, rng = 1024, random.Random(3)
+    c, book = new_cache(env, (16, 1, 64, 64, True), layers=1, pages=4100, seqs=2 * n, cols=4)
+    order = rng.sample(range(n), n)
+    counts = [rng.choice((0, 1, 2, 16, 30)) for _ in order]
+    lib.cache_reserve(c, starts_of(env, counts), ints(env, order))
+    book.reserve(order, counts)
+    kids = [n + s for s in order]
+    lib.cache_fork(c, ints(env, order), ints(env, kids))
+    book.fork(order, kids)
+    image = c.pages.clone()
+    some = rng.sample(kids, n)
+    more = [rng.choice((0, 1, 3, 17)) for _ in some]
+    lib.cache_reserve(c, starts_of(env, more), ints(env, some))
+    image = moved(image, book.reserve(some, more))
+    check(env, c, book, image)
+    # appended as one list, and one sequence after the other
+    k, v = rows(env, sum(more), c, 6)
+    starts = starts_of(env, more)
+    for i, s in enumerate(some[:300]):
+        lib.cache_append(c, 0, k, v, starts[i:i + 2].contiguous(), ints(env, [s]))
+    rest = starts[300:].contiguous()
+    lib.cache_append(c, 0, k, v, rest, ints(env, some[300:]))
+    want = c.pages.clone()
+    c.pages.copy_(image)
+    lib.cache_append(c, 0, k, v, starts, ints(env, some))
+    assert lib.cache_status(c) == 0 and torch.equal(c.pages, want)
+    c.pages.copy_(image)
+    for at in (1, 63, 64, 65, 128, 1000, 1023):  # starts that fall there
+        bad = starts.clone()
+        bad[at] = bad[at - 1] - 1 if at > 1 else bad[at + 1] + 1
+        lib.cache_append(c, 0, k, v, bad, ints(env, some))
+        assert lib.cache_status(c) == LIST and torch.equal(c.pages, image), at
+    for i, j in ((0, 64), (63, 1023), (5, 6)):   # a sequence twice
+        twice = list(some)
+        twice[j] = twice[i]
+        lib.cache_append(c, 0, k, v, starts, ints(env, twice))
+        want_bit = LIST if more[i] or more[j] else 0
+        assert lib.cache_status(c) == want_bit
+        for entry in (i, j):
+            page = {p for p in book.table[some[entry]] if p >= 0}
+            for p in page:
+                if book.ref[p] == 1:
+                    assert torch.equal(c.pages[:, p], image[:, p]), (i, j, entry)
+        c.pages.copy_(image)
+    to = [rng.randint(0, book.len[s]) for s in some]
+    lib.cache_free(c, ints(env, some), ints(env, to))
+    book.free(some, to)
+    check(env, c, book, image)
