@@ -25,19 +25,20 @@
 // per 16 lanes.
 //
 // What bounds it, with 64 latent heads of 512 if nothing else is said:
-//  - a chunk of 2048 tokens behind 14336, BF16: 3.8 to 3.95 ms, 1.04 to 1.09
-//    PFLOP/s, 79 to 83% of a large library product's rate; the matrix unit is
+//  - a chunk of 2048 tokens behind 14336, BF16: 3.8 to 4.1 ms, 1.0 to 1.09
+//    PFLOP/s, 77 to 83% of a large library product's rate; the matrix unit is
 //    busy 45% of the time. Without the loads in the loop it would take 3.1 ms;
-//    half of the LDS reads changed nothing. E4M3 4.6 ms (the conversion).
-//  - decode over long caches: HBM. 64 sequences of 8100: BF16 130 us (4.1 TB/s),
-//    E4M3 127 to 145 us (the conversion: half the bytes, the same LDS traffic);
-//    8 sequences of 16000 over 8 kv heads of 128, BF16: 103 us, 5.1 TB/s.
+//    half of the LDS reads changed nothing. E4M3 4.4 to 4.6 ms (the conversion).
+//  - decode over long caches: HBM. 64 sequences of 8100: BF16 124 to 152 us (3.6
+//    to 4.4 TB/s), E4M3 126 to 145 us (the conversion: half the bytes, the same
+//    LDS traffic); 8 sequences of 16000 over 8 kv heads of 128, BF16: 103 us, 5.1 TB/s.
 //  - short ones: dependent latencies. One sequence of 1777: 18 us, of which
 //    finding the place 2.6, the item and its pages 2, the query rows 2.7, the
 //    first rows of the cache 1.4, the stages 2.2, the waves' exchange 3.1, the
 //    parts' stores 1.3; the launch that joins them 5.5.
 // Taken back: query rows asked for before the second stage's loads (a chunk 2%
-// faster, decode 1 to 3% slower), query rows first of all (spills).
+// faster, decode 1 to 3% slower), query rows first of all (spills), weights by a
+// branch on the scores' size (latent decode 3 to 8% slower, a chunk 3%).
 #include <algorithm>
 #include <cmath>
 #include <utility>
@@ -676,7 +677,7 @@ __global__ __launch_bounds__(256, (Cfg<D, SHARED, FP8, RW>::WGS)) void k_attn(DS
     int id = blockIdx.x;
     w.kvh = id % C.kv_heads;
     id /= C.kv_heads;
-    // the longest ranges first
+    // of each sequence the longest ranges first
     w.pair = id % a.n_seqs * a.tiles + a.tiles - 1 - id / a.n_seqs;
     w.stage = 0;
     w.at = 0;

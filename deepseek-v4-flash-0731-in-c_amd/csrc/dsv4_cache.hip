@@ -77,8 +77,8 @@ __global__ void k_cache_clear_status(unsigned *status) { *status = 0; }
 // the pages it needs, the pool is scanned from its start until enough free
 // pages are found, and only then anything is changed. One workgroup; bound by
 // the latency of its dependent steps (list -> length -> table -> ref -> scan):
-// 9.4 us for 16 sequences and 512 pages, and no less with the counts loaded
-// ahead.
+// 9.4 to 10.5 us for 16 sequences and 512 pages, and no less with the counts
+// loaded ahead.
 __global__ __launch_bounds__(CB_T) void k_cache_reserve(DSV4GCache C, const int *seqs,
                                                         const int *starts, int n, int *ws) {
   __shared__ int s_seq[CB_T], s_page[CB_T], s_off[CB_T], s_at[CB_T], s_copy[CB_T];
@@ -357,8 +357,8 @@ __global__ __launch_bounds__(CB_T) void k_cache_compact(DSV4GCache C, int *n_use
 // One wave per new token: its place by counting the starts at or before its
 // row, then 8 columns per lane and step (8 neighbouring lanes are one scale
 // group of 64 columns). Bound: HBM for many tokens (4096 of 8 kv heads of 128
-// and 128: 53 MB in 11.3 us, 4.7 TB/s), the latency of starts -> sequence ->
-// length -> table entry -> store for few (64 latent rows: 4.2 us).
+// and 128: 53 MB in 11.8 to 12.1 us, 4.5 TB/s), the latency of starts -> sequence
+// -> length -> table entry -> store for few (64 latent rows: 4.1 to 4.6 us).
 template <bool F32, bool FP8>
 __global__ __launch_bounds__(256) void k_cache_append(DSV4GCache C, CacheGeom G, int layer,
                                                       const void *k, size_t k_stride,

@@ -32,12 +32,12 @@
 // the larger of a[i] and b[63 - i] is the upper half of both, a bitonic sequence.
 //
 // Bound: HBM for fp32 rows (2048 rows of 129280: 179 us, 5.9 TB/s), the vector
-// units for BF16 ones, with half the bytes per value (125 us, 4.2 TB/s: about 10
-// instructions a value, one of them 2^x at a quarter of the rate; with the
-// index compared for every value's rank it was 156). k = 8 adds 15 and 59 us: a
-// wave looks through its first tiles and then ever fewer. Fewer registers for
-// it (six waves per SIMD in place of five) cost 10%: the sort's lane masks are
-// then computed at each use.
+// units for BF16 ones, with half the bytes per value (107 to 117 us, 4.5 to 4.9
+// TB/s: about 10 instructions a value, one of them 2^x at a quarter of the rate;
+// the index compared for every value's rank cost a quarter more). k = 8 adds 15
+// and 37 us: a wave looks through its first tiles and then ever fewer. Fewer
+// registers for it (six waves per SIMD in place of five) cost 10%: the sort's lane
+// masks are then computed at each use.
 // Rows are cut into segments until a launch has about 2048 workgroups, what the
 // chip holds at once; a second launch joins them (64 rows 12 us, one row 17 us,
 // against 278 and 303 us in library calls).

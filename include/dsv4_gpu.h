@@ -380,9 +380,10 @@ int dsv4g_ffn_step(float *state, const float *hc_fn, const float *hc_scale,
  * DSV4G_DT_BF16: two bytes each. DSV4G_DT_F8_E4M3: one code each, then in the
  * same order an E8M0 code per DSV4G_CACHE_GROUP columns
  * ([kv_heads][page_size][k_dim / 64], the values' after them); a value is
- * code * 2^(scale - 127) (a scale code of 255 counts as 254; append writes
- * 105 .. 247). A page takes dsv4g_cache_page_bytes(C), a multiple
- * of 256; page p of layer l is at pages + (l * n_pages + p) * that.
+ * code * 2^(scale - 127) as BF16, infinite beyond its range (a scale code of 255
+ * counts as 254; append writes 105 .. 247). A page takes
+ * dsv4g_cache_page_bytes(C), a multiple of 256; page p of layer l is at
+ * pages + (l * n_pages + p) * that.
  *
  * Sequence s (a row of the table) holds len[s] tokens; its j-th token lies in
  * page table[s][j / page_size]. Entries behind its pages are -1. ref[p] counts
@@ -479,7 +480,8 @@ int dsv4g_cache_compact(const DSV4GCache *C, int *n_used, void *workspace,
  * summed in fp32 and must stay in its range; |scale| is at most 2.35e38.
  * Tokens that a row does not see have no influence on it, whatever they hold;
  * a row that sees a key or value that is not finite is not finite in the
- * columns concerned (which others are not is left open).
+ * columns concerned (which others are not is left open; a token whose score
+ * is -inf weighs nothing).
  * q [n_tokens][heads][k_dim] with q_stride elements from token to token, out
  * [n_tokens][heads][v_dim or k_dim] with out_stride, both act_dtype:
  * DSV4G_DT_BF16, or DSV4G_DT_F32 holding BF16 values as every activation here
