@@ -653,3 +653,26 @@ def test_products_at_both_ends_of_fp32(env, shape):
                 tol, tol_lse = paged.attend_bounds(o, mass, torch.zeros_like(e), kd)
                 assert ((out[r] - o).abs() <= tol).all(), (scale, kv, r)
                 assert ((lse[r] - e).abs() <= tol_lse).all(), (scale, kv, r)
+
+
+@pytest.mark.parametrize("kv", [102, 65536])
+def test_sinks_that_are_not_finite(env, kv):
+    """A sink of -inf is none, one of inf takes everything, a NaN is one; heads
+    beside them are as without."""
+    torch, lib, dev = env["torch"], env["lib"], env["dev"]
+    s = Setup(env, GQA, 16, False, [100, 0], [2, 1], seed=24)
+    c = wide_table(s)
+    run = lambda sink: lib.attention(c, 1, s.q, s.starts, max_q=2, max_kv=kv, sink=sink,  # noqa: E731
+                                     with_lse=True)
+    plain, plain_lse = run(None)
+    sink = torch.full((32,), float("-inf"), device=dev)
+    out, lse = run(sink)
+    assert torch.equal(out, plain) and torch.equal(lse, plain_lse)
+    sink[3], sink[17] = float("inf"), float("nan")
+    out, lse = run(sink)
+    others = [h for h in range(32) if h not in (3, 17)]
+    assert torch.equal(out[:, others], plain[:, others])
+    assert torch.equal(lse[:, others], plain_lse[:, others])
+    assert (out[:, 3] == 0).all() and (lse[:, 3] == float("inf")).all()
+    assert out[:, 17].isnan().all() and lse[:, 17].isnan().all()
+    assert lib.cache_status(c) == 0
