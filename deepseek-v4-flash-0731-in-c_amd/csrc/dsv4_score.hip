@@ -6,10 +6,9 @@
 // keeps the running maximum m of its z and, with M = fl(m L),
 //   s = sum 2^(z L - M),  t = sum 2^(z L - M) (z L - M)
 // (one fma and the hardware's 2^x per logit). Where |M| is SC_NEAR or more (masks
-// of -10^9 and beyond, in a thread that has seen nothing else, or the largest of
-// logits), M's rounding would grow until no 2^x holds it: there the exponent is
-// (z - m) L, one instruction more (taken everywhere, it costs 4% of 2048 BF16
-// rows). With off(m) what the first kind of M is off m L, exactly by an fma, two
+// beyond -45000 in a thread that has seen nothing else, or logits as large), M's
+// rounding would grow until no 2^x holds it: there the exponent is (z - m) L, one
+// instruction more (taken everywhere, it costs 4% of 2048 BF16 rows). With off(m) what the first kind of M is off m L, exactly by an fma, two
 // triples join as
 //   m' = max(m1, m2),  g = (m1 - m') L + off(m1) - off(m'),  f = 2^g,
 //   s' = f s1 + ..,    t' = f (t1 + g s1) + ..
@@ -286,7 +285,7 @@ __global__ __launch_bounds__(SC_T) void k_score(ScoreArgs a) {
     const T e = l[token];
     zt = (sizeof(T) == 4 ? u2f((uint32_t)e) : u2f((uint32_t)e << 16)) * a.scale;
   }
-  // the next value below it: below 0 that is behind -0, which no order holds
+  // the next value below it (of 0: past -0, which the order has no place for)
   const float zt_below = unordered(ordered(zt) - (zt == 0.0f ? 2 : 1));
   if (TOP) {
     if (tid < 4) s_bar[tid] = -__builtin_inff();
